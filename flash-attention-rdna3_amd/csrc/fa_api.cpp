@@ -119,6 +119,10 @@ size_t fa_params_size(int which) {
     case 3: return sizeof(fa_paged_params);
     case 4: return sizeof(fa_tiny_params);
     case 5: return sizeof(fa_append_params);
+    case 6: return sizeof(fa_paged_blocks_params);
+    case 7: return sizeof(fa_allocate_params);
+    case 8: return sizeof(fa_paged_append_params);
+    case 9: return sizeof(fa_select_params);
   }
   return 0;
 }
@@ -334,6 +338,77 @@ int fa_kvcache_append(const fa_append_params* params, void* stream) {
       !rows_ok(p.k_cache, p.k_cache_stride, 4, 2) || !rows_ok(p.v_cache, p.v_cache_stride, 4, 2))
     return fail(FA_ERR_INVALID, "fa_kvcache_append: tensors need a unit last stride and 16-byte aligned rows");
   return from_hip(fa::launch_append(p, (hipStream_t)stream), "fa_kvcache_append");
+}
+
+namespace {
+
+bool block_size_ok(int n) { return n >= 1 && n <= 256 && (n & (n - 1)) == 0; }
+
+// A grid's second and third extents.
+bool grid_ok(int64_t n) { return n <= 65535; }
+
+}  // namespace
+
+int fa_paged_allocate(const fa_allocate_params* params, void* stream) {
+  if (!params) return fail(FA_ERR_INVALID, "fa_paged_allocate: params is NULL");
+  const fa_allocate_params& p = *params;
+  if (p.abi_version != FA_ABI_VERSION) return fail(FA_ERR_INVALID, "fa_paged_allocate: abi_version mismatch");
+  if (p.batch <= 0 || p.max_blocks <= 0 || p.num_free < 0 || p.num_tokens < 0 || !block_size_ok(p.block_size))
+    return fail(FA_ERR_INVALID, "fa_paged_allocate: bad shape");
+  if (!p.block_table || !p.context_lens || !p.new_lens || (p.num_free > 0 && !p.free_blocks) ||
+      (p.num_tokens > 0 && !p.slots) || !p.cu_seqlens || !p.next_head)
+    return fail(FA_ERR_INVALID, "fa_paged_allocate: NULL tensor");
+  return from_hip(fa::launch_allocate(p, (hipStream_t)stream), "fa_paged_allocate");
+}
+
+int fa_paged_append(const fa_paged_append_params* params, void* stream) {
+  if (!params) return fail(FA_ERR_INVALID, "fa_paged_append: params is NULL");
+  const fa_paged_append_params& p = *params;
+  if (p.abi_version != FA_ABI_VERSION) return fail(FA_ERR_INVALID, "fa_paged_append: abi_version mismatch");
+  if (p.dtype != FA_DTYPE_F16 && p.dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_INVALID, "fa_paged_append: dtype must be f16 or bf16");
+  if (p.kv_format < FA_KV_SAME || p.kv_format > FA_KV_INT8)
+    return fail(FA_ERR_INVALID, "fa_paged_append: kv_format %d", p.kv_format);
+  if (!dim_ok(p.head_dim) && !(p.head_dim == 16 && p.kv_format == FA_KV_SAME))
+    return fail(FA_ERR_UNSUPPORTED, "fa_paged_append: head_dim %d", p.head_dim);
+  if (p.num_tokens < 0 || p.heads_kv <= 0 || p.num_blocks <= 0 || !block_size_ok(p.block_size) ||
+      !grid_ok(2 * (int64_t)p.heads_kv))
+    return fail(FA_ERR_INVALID, "fa_paged_append: bad shape");
+  if (p.num_tokens == 0) return FA_OK;
+  const int es = p.kv_format == FA_KV_SAME ? 2 : 1;
+  if (!rows_ok(p.k_new, p.k_new_stride, 3, 2) || !rows_ok(p.v_new, p.v_new_stride, 3, 2) ||
+      !rows_ok(p.k_cache, p.k_cache_stride, 4, es) || !rows_ok(p.v_cache, p.v_cache_stride, 4, es) ||
+      (p.key_bounds && !rows_ok(p.key_bounds, p.bounds_stride, 4, 2)))
+    return fail(FA_ERR_INVALID, "fa_paged_append: tensors need a unit last stride and 16-byte aligned rows");
+  if (!p.slots) return fail(FA_ERR_INVALID, "fa_paged_append: slots is NULL");
+  if (p.kv_format != FA_KV_SAME && (!p.k_scale || !p.v_scale))
+    return fail(FA_ERR_INVALID, "fa_paged_append: an 8-bit cache needs k_scale and v_scale");
+  return from_hip(fa::launch_paged_append(p, (hipStream_t)stream), "fa_paged_append");
+}
+
+size_t fa_select_workspace_bytes(int batch, int heads_kv, int max_blocks) {
+  if (batch <= 0 || heads_kv <= 0 || max_blocks <= 0) return 0;
+  return fa::select_workspace_bytes(batch, heads_kv, max_blocks);
+}
+
+int fa_paged_select(const fa_select_params* params, void* stream) {
+  if (!params) return fail(FA_ERR_INVALID, "fa_paged_select: params is NULL");
+  const fa_select_params& p = *params;
+  if (p.abi_version != FA_ABI_VERSION) return fail(FA_ERR_INVALID, "fa_paged_select: abi_version mismatch");
+  if (p.dtype != FA_DTYPE_F16 && p.dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_INVALID, "fa_paged_select: dtype must be f16 or bf16");
+  if (!dim_ok(p.head_dim)) return fail(FA_ERR_UNSUPPORTED, "fa_paged_select: head_dim %d", p.head_dim);
+  if (p.batch <= 0 || p.heads_q <= 0 || p.heads_kv <= 0 || p.heads_q % p.heads_kv || p.seqlen_q <= 0 ||
+      p.num_blocks <= 0 || p.max_blocks <= 0 || !block_size_ok(p.block_size) || p.n_index <= 0 || !grid_ok(p.batch) ||
+      !grid_ok(p.heads_kv))
+    return fail(FA_ERR_INVALID, "fa_paged_select: bad shape");
+  if (p.keep_first < 0 || p.keep_last < 0 || (int64_t)p.keep_first + p.keep_last > p.n_index)
+    return fail(FA_ERR_INVALID, "fa_paged_select: keep_first + keep_last must lie in 0..n_index");
+  if (!rows_ok(p.q, p.q_stride, 4, 2) || !rows_ok(p.key_bounds, p.bounds_stride, 4, 2))
+    return fail(FA_ERR_INVALID, "fa_paged_select: q and key_bounds need a unit last stride and 16-byte aligned rows");
+  if (!p.block_table || !p.context_lens || !p.index) return fail(FA_ERR_INVALID, "fa_paged_select: NULL tensor");
+  if (!p.workspace || !aligned16(p.workspace)) return fail(FA_ERR_INVALID, "fa_paged_select: workspace");
+  return from_hip(fa::launch_select(p, (hipStream_t)stream), "fa_paged_select");
 }
 
 }  // extern "C"

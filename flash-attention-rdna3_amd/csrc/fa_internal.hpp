@@ -41,6 +41,10 @@ hipError_t launch_decode_noalloc(const fa_decode_params& p, hipStream_t stream);
 hipError_t launch_paged(const fa_paged_params& p, hipStream_t stream);
 hipError_t launch_tiny(const fa_tiny_params& p, hipStream_t stream);
 hipError_t launch_append(const fa_append_params& p, hipStream_t stream);
+hipError_t launch_allocate(const fa_allocate_params& p, hipStream_t stream);
+hipError_t launch_paged_append(const fa_paged_append_params& p, hipStream_t stream);
+hipError_t launch_select(const fa_select_params& p, hipStream_t stream);
+size_t select_workspace_bytes(int batch, int heads_kv, int max_blocks);
 
 size_t decode_workspace_bytes(int batch, int heads_q, int seqlen_q, int head_dim, int num_splits);
 

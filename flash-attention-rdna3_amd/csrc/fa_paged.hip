@@ -1,0 +1,673 @@
+// fa_paged.hip - block tables and slot maps, appends to a paged cache, and the
+// choice of blocks by their key bounds, for gfx950.  The attention that reads
+// such a cache is in fa_paged_attn.hpp.
+//
+// The reference takes ready tables and a filled 16-bit cache
+// (fa_rdna3/interface.py:643-728); nothing here has a counterpart there.
+#include "fa_internal.hpp"
+#include "fa_tiles.hpp"
+
+namespace fa {
+
+// ---------------------------------------------------------------------------
+// Block tables and slot maps.
+//
+// With P = block_size and cap = max_blocks * P, sequence b owns the blocks
+// [0, first_b) and needs [first_b, last_b), first_b = ceil(min(ctx, cap) / P),
+// last_b = ceil(min(ctx + new, cap) / P); its new blocks are the free list's
+// entries [start_b, start_b + last_b - first_b), start_b the running sum of
+// what the sequences before it need.  The first position of a new block is
+// always a new token (first_b * P >= ctx), so the thread of that token enters
+// the block into the table: no thread reads an entry that another one writes.
+//
+// One launch, no communication between workgroups: each sums the lengths
+// again (8 bytes a sequence, from L2 after the first) in windows of kSeqs
+// sequences held in LDS, and looks its tokens' sequences up there.
+// ---------------------------------------------------------------------------
+namespace {
+constexpr int kAllocThreads = 256;
+constexpr int kSeqs = 1024;  // sequences of a window
+}  // namespace
+
+__global__ __launch_bounds__(kAllocThreads) void paged_allocate_kernel(fa_allocate_params p, int shift) {
+  __shared__ int64_t tok_end[kSeqs];    // running sum of new tokens, sequence included
+  __shared__ int64_t blk_start[kSeqs];  // running sum of needed blocks, sequence excluded
+  __shared__ int64_t wave_tok[4], wave_blk[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t P = p.block_size, cap = (int64_t)p.max_blocks * P;
+  const int64_t head = p.free_head ? max(*p.free_head, 0) : 0;
+  const int64_t stride = (int64_t)gridDim.x * kAllocThreads;
+  int64_t tok_base = 0, blk_base = 0;
+  int64_t t = (int64_t)blockIdx.x * kAllocThreads + tid;  // this thread's next token
+  for (int b0 = 0; b0 < p.batch; b0 += kSeqs) {
+    constexpr int PER = kSeqs / kAllocThreads;
+    int64_t tok[PER], blk[PER], tsum = 0, bsum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int b = b0 + tid * PER + i;
+      int64_t ctx = 0, add = 0;
+      if (b < p.batch) {
+        ctx = max(p.context_lens[b * p.context_lens_stride], 0);
+        add = max(p.new_lens[b * p.new_lens_stride], 0);
+      }
+      const int64_t first = (min(ctx, cap) + P - 1) >> shift, last = (min(ctx + add, cap) + P - 1) >> shift;
+      blk[i] = bsum;
+      tsum += add;
+      bsum += last - first;
+      tok[i] = tsum;
+    }
+    int64_t ti = tsum, bi = bsum;  // inclusive over the wave's lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t ty = __shfl_up(ti, o, 64), by = __shfl_up(bi, o, 64);
+      if (lane >= o) { ti += ty; bi += by; }
+    }
+    if (lane == 63) { wave_tok[wave] = ti; wave_blk[wave] = bi; }
+    __syncthreads();
+    int64_t tprev = tok_base + ti - tsum, bprev = blk_base + bi - bsum, tall = 0, ball = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) { tprev += wave_tok[w]; bprev += wave_blk[w]; }
+      tall += wave_tok[w];
+      ball += wave_blk[w];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      tok_end[tid * PER + i] = tprev + tok[i];
+      blk_start[tid * PER + i] = bprev + blk[i];
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+      if (b0 == 0 && tid == 0) p.cu_seqlens[0] = 0;
+      for (int i = tid; i < kSeqs && b0 + i < p.batch; i += kAllocThreads) p.cu_seqlens[b0 + i + 1] = (int32_t)tok_end[i];
+    }
+    tok_base += tall;
+    blk_base += ball;
+    for (; t < tok_base; t += stride) {
+      int lo = 0, hi = min(kSeqs, p.batch - b0) - 1;  // the first sequence that ends past t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (tok_end[mid] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int b = b0 + lo;
+      const int64_t ctx = max(p.context_lens[b * p.context_lens_stride], 0);
+      const int64_t add = max(p.new_lens[b * p.new_lens_stride], 0);
+      const int64_t pos = ctx + (t - (tok_end[lo] - add));
+      int64_t slot = -1;
+      if (pos < cap) {
+        const int64_t blk_at = pos >> shift, first = (min(ctx, cap) + P - 1) >> shift;
+        int32_t* const entry = p.block_table + b * p.block_table_stride[0] + blk_at * p.block_table_stride[1];
+        int32_t page;
+        if (blk_at < first) {
+          page = *entry;
+        } else {
+          const int64_t at = head + blk_start[lo] + (blk_at - first);
+          page = at < p.num_free ? p.free_blocks[at * p.free_blocks_stride] : -1;
+          if ((pos & (P - 1)) == 0) *entry = page;
+        }
+        if (page >= 0) slot = (int64_t)page * P + (pos & (P - 1));
+      }
+      if (t < p.num_tokens) p.slots[t] = slot;
+    }
+    __syncthreads();  // the next window writes the arrays
+  }
+  for (; t < p.num_tokens; t += stride) p.slots[t] = -1;
+  if (blockIdx.x == 0 && tid == 0) p.next_head[0] = (int32_t)(head + blk_base);
+}
+
+static int log2_of(int n) {
+  int s = 0;
+  while ((1 << s) < n) ++s;
+  return s;
+}
+
+hipError_t launch_allocate(const fa_allocate_params& p, hipStream_t stream) {
+  const int64_t want = ((int64_t)p.num_tokens + 4 * kAllocThreads - 1) / (4 * kAllocThreads);
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>(want, 1), 1024);
+  hipLaunchKernelGGL(paged_allocate_kernel, dim3(grid), dim3(kAllocThreads), 0, stream, p, log2_of(p.block_size));
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Append.  The tokens of one block (a segment: they lie within P consecutive
+// rows, between them at most dropped ones) are one wave's work for each head
+// of K and of V: lanes own 8 dims (16 bytes) of a row, D / 8 lanes a row, and
+// 512 / D rows go at a time.  The wave of the segment's first row does it all;
+// the P rows before tell whether a row is the first.
+//
+// 8-bit rows are x / s with s a power of two, so the quotient is exact and a
+// value is rounded once, when it is stored; a block whose scale grows rounds
+// its rows again on the coarser grid.  Scales of any value would round every
+// row again whenever a slightly larger value arrived.
+// ---------------------------------------------------------------------------
+namespace {
+constexpr int kAppendWaves = 4;
+
+struct AppendSide {
+  const uint16_t* src;
+  void* dst;
+  float* scale;
+  int64_t src_stride[2];  // token, head
+  int64_t dst_stride[3];  // block, position, head
+  int64_t scale_stride[2];
+};
+
+struct AppendArgs {
+  AppendSide side[2];  // K, V
+  const int64_t* slots;
+  int64_t slots_stride;
+  uint16_t* bounds;
+  int64_t bounds_stride[3];  // block, head, low / high
+  int32_t num_tokens, heads_kv, num_blocks, shift, chunk;
+};
+
+template <int FMT> struct Code;
+template <> struct Code<FA_KV_E4M3> {
+  static constexpr float kTop = 448.f;
+  static constexpr int kTopExp = 8;
+  static constexpr uint32_t kTopMant = 0x600000u;
+  // Four codes of |x| <= 448 or NaN.
+  __device__ static uint32_t pack(const float* x) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+  }
+  __device__ static void unpack(uint32_t w, float* x) {
+    x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+    x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+    x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+    x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+  }
+};
+template <> struct Code<FA_KV_INT8> {
+  static constexpr float kTop = 127.f;
+  static constexpr int kTopExp = 6;
+  static constexpr uint32_t kTopMant = 0x7E0000u;
+  __device__ static uint32_t pack(const float* x) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= ((uint32_t)(int)(x[i] == x[i] ? rintf(x[i]) : 0.f) & 0xFFu) << (8 * i);
+    return w;
+  }
+  __device__ static void unpack(uint32_t w, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+  }
+};
+
+// x clamped to +-top; NaN stays NaN.
+template <int FMT> __device__ inline float clamp_code(float x) {
+  return x == x ? fminf(fmaxf(x, -Code<FMT>::kTop), Code<FMT>::kTop) : x;
+}
+
+// The least power of two 2^e, e >= -100, with amax <= top * 2^e.
+template <int FMT> __device__ inline float scale_for(float amax) {
+  using C = Code<FMT>;
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = (int)(bits >> 23) - 127 - C::kTopExp + ((bits & 0x7FFFFFu) > C::kTopMant ? 1 : 0);
+  return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
+}
+}  // namespace
+
+template <typename Tag, int FMT, int D>
+__global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendArgs a) {
+  using EL = Elem<Tag>;
+  constexpr int LPR = D / 8;    // lanes of a row
+  constexpr int RPI = 64 / LPR; // rows at a time
+  extern __shared__ int32_t staged[];  // page, position of the chunk's tokens and those behind it
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int P = 1 << a.shift;
+  const int64_t t0 = (int64_t)blockIdx.x * a.chunk;
+  // Token t0 - P + i at entry i: the chunk, and P rows before and behind it.
+  const int span = a.chunk + 2 * P;
+  int32_t* const page_of = staged;
+  int32_t* const pos_of = staged + span;
+  for (int i = tid; i < span; i += 64 * kAppendWaves) {
+    const int64_t t = t0 - P + i;
+    int32_t page = -1, pos = 0;
+    if (t >= 0 && t < a.num_tokens) {
+      const int64_t slot = a.slots[t * a.slots_stride];
+      if (slot >= 0 && (slot >> a.shift) < a.num_blocks) {
+        page = (int32_t)(slot >> a.shift);
+        pos = (int32_t)(slot & (P - 1));
+      }
+    }
+    page_of[i] = page;
+    pos_of[i] = pos;
+  }
+  __syncthreads();
+  const int item = blockIdx.y * kAppendWaves + wave;
+  if (item >= 2 * a.heads_kv) return;
+  const int head = item >> 1;
+  const AppendSide& s = a.side[item & 1];
+  const int c = lane % LPR, sub = lane / LPR;
+  // Page of the last row that is not dropped, within the P rows before.
+  int prev = -1, prev_at = -1;
+  for (int i0 = 0; i0 < P; i0 += 64) {
+    const uint64_t kept = __builtin_amdgcn_ballot_w64(i0 + lane < P && page_of[i0 + lane] >= 0);
+    if (kept) prev_at = i0 + 63 - __builtin_clzll(kept);
+  }
+  if (prev_at >= 0) prev = __builtin_amdgcn_readfirstlane(page_of[prev_at]);
+  for (int i = P; i < P + a.chunk; ++i) {
+    const int page = __builtin_amdgcn_readfirstlane(page_of[i]);
+    if (page < 0) continue;
+    const bool goes_on = page == prev && i - prev_at < P;
+    prev = page;
+    prev_at = i;
+    if (goes_on) continue;
+    // The segment: rows i .. i + n - 1 but for dropped ones, and its lowest position.
+    int n = P, lowest = P;
+    for (int j0 = 0; j0 < P; j0 += 64) {
+      const int j = j0 + lane;
+      const int at = j < P ? page_of[i + j] : -1;
+      const uint64_t other = __builtin_amdgcn_ballot_w64(at >= 0 && at != page);
+      if (other) n = min(n, j0 + (int)__builtin_ctzll(other));
+      if (at == page && j < n) lowest = min(lowest, pos_of[i + j]);
+      if (other) break;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) lowest = min(lowest, __shfl_xor(lowest, o, 64));
+    lowest = __builtin_amdgcn_readfirstlane(lowest);
+    const uint16_t* const src = s.src + (t0 - P + i) * s.src_stride[0] + head * s.src_stride[1] + 8 * c;
+    auto mine = [&](int r) { return page_of[i + r] == page; };
+    auto row_of = [&](int r) { return *reinterpret_cast<const s16x8*>(src + r * s.src_stride[0]); };
+
+    if (a.bounds && (item & 1) == 0) {
+      float low[8], high[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { low[e] = -kNegInf; high[e] = kNegInf; }
+      uint16_t* const bl = a.bounds + page * a.bounds_stride[0] + head * a.bounds_stride[1] + 8 * c;
+      uint16_t* const bh = bl + a.bounds_stride[2];
+      if (lowest > 0 && sub == 0) {
+        const s16x8 x = *reinterpret_cast<const s16x8*>(bl), y = *reinterpret_cast<const s16x8*>(bh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { low[e] = EL::to_f((uint16_t)x[e]); high[e] = EL::to_f((uint16_t)y[e]); }
+      }
+      for (int r = sub; r < n; r += RPI) {
+        if (!mine(r)) continue;
+        const s16x8 x = row_of(r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = EL::to_f((uint16_t)x[e]);
+          low[e] = fminf(low[e], f);   // (a NaN operand leaves the other)
+          high[e] = fmaxf(high[e], f);
+        }
+      }
+#pragma unroll
+      for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          low[e] = fminf(low[e], __shfl_xor(low[e], o, 64));
+          high[e] = fmaxf(high[e], __shfl_xor(high[e], o, 64));
+        }
+      if (sub == 0) {
+        s16x8 x, y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { x[e] = (short)EL::from_f(low[e]); y[e] = (short)EL::from_f(high[e]); }
+        *reinterpret_cast<s16x8*>(bl) = x;
+        *reinterpret_cast<s16x8*>(bh) = y;
+      }
+    }
+
+    if constexpr (FMT == FA_KV_SAME) {
+      uint16_t* const dst = reinterpret_cast<uint16_t*>(s.dst) + page * s.dst_stride[0] + head * s.dst_stride[2] + 8 * c;
+      for (int r = sub; r < n; r += RPI)
+        if (mine(r)) *reinterpret_cast<s16x8*>(dst + pos_of[i + r] * s.dst_stride[1]) = row_of(r);
+    } else {
+      using C = Code<FMT>;
+      float amax = 0.f;
+      for (int r = sub; r < n; r += RPI) {
+        if (!mine(r)) continue;
+        const s16x8 x = row_of(r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = fabsf(EL::to_f((uint16_t)x[e]));
+          amax = fmaxf(amax, f < __builtin_inff() ? f : 0.f);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+      float* const scale = s.scale + page * s.scale_stride[0] + head * s.scale_stride[1];
+      const float before = lowest > 0 ? *scale : 0.f;
+      const float after = fmaxf(before, scale_for<FMT>(amax));
+      uint8_t* const dst = reinterpret_cast<uint8_t*>(s.dst) + page * s.dst_stride[0] + head * s.dst_stride[2] + 8 * c;
+      if (lowest > 0 && after > before) {
+        const float ratio = before / after;
+        for (int r = sub; r < lowest; r += RPI) {
+          u32x2* const at = reinterpret_cast<u32x2*>(dst + r * s.dst_stride[1]);
+          const u32x2 w = *at;
+          u32x2 z;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[4];
+            C::unpack(w[h], x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] *= ratio;
+            z[h] = C::pack(x);
+          }
+          *at = z;
+        }
+      }
+      const float inv = 1.f / after;
+      for (int r = sub; r < n; r += RPI) {
+        if (!mine(r)) continue;
+        const s16x8 x = row_of(r);
+        u32x2 z;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = clamp_code<FMT>(EL::to_f((uint16_t)x[4 * h + e]) * inv);
+          z[h] = C::pack(f);
+        }
+        *reinterpret_cast<u32x2*>(dst + pos_of[i + r] * s.dst_stride[1]) = z;
+      }
+      if (lane == 0) *scale = after;
+    }
+  }
+}
+
+template <typename Tag, int FMT, int D>
+static hipError_t run_append(const AppendArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.num_tokens + a.chunk - 1) / a.chunk), (2 * a.heads_kv + kAppendWaves - 1) / kAppendWaves);
+  hipLaunchKernelGGL((paged_append_kernel<Tag, FMT, D>), grid, dim3(64 * kAppendWaves),
+                     2 * (a.chunk + (2 << a.shift)) * sizeof(int32_t), stream, a);
+  return hipGetLastError();
+}
+
+template <typename Tag, int FMT>
+static hipError_t append_by_dim(const AppendArgs& a, int dim, hipStream_t stream) {
+  switch (dim) {
+    case 16: return FMT == FA_KV_SAME ? run_append<Tag, FA_KV_SAME, 16>(a, stream) : hipErrorInvalidValue;
+    case 32: return run_append<Tag, FMT, 32>(a, stream);
+    case 64: return run_append<Tag, FMT, 64>(a, stream);
+    case 128: return run_append<Tag, FMT, 128>(a, stream);
+    case 256: return run_append<Tag, FMT, 256>(a, stream);
+    case 512: return run_append<Tag, FMT, 512>(a, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+template <typename Tag>
+static hipError_t append_by_format(const AppendArgs& a, int format, int dim, hipStream_t stream) {
+  switch (format) {
+    case FA_KV_SAME: return append_by_dim<Tag, FA_KV_SAME>(a, dim, stream);
+    case FA_KV_E4M3: return append_by_dim<Tag, FA_KV_E4M3>(a, dim, stream);
+    case FA_KV_INT8: return append_by_dim<Tag, FA_KV_INT8>(a, dim, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_paged_append(const fa_paged_append_params& p, hipStream_t stream) {
+  if (p.num_tokens == 0) return hipSuccess;
+  AppendArgs a{};
+  auto side = [&](AppendSide& s, const void* src, void* dst, float* scale, const int64_t* ss, const int64_t* ds,
+                  const int64_t* cs) {
+    s.src = reinterpret_cast<const uint16_t*>(src);
+    s.dst = dst;
+    s.scale = scale;
+    for (int i = 0; i < 2; ++i) s.src_stride[i] = ss[i];
+    for (int i = 0; i < 3; ++i) s.dst_stride[i] = ds[i];
+    for (int i = 0; i < 2; ++i) s.scale_stride[i] = cs[i];
+  };
+  side(a.side[0], p.k_new, p.k_cache, p.k_scale, p.k_new_stride, p.k_cache_stride, p.k_scale_stride);
+  side(a.side[1], p.v_new, p.v_cache, p.v_scale, p.v_new_stride, p.v_cache_stride, p.v_scale_stride);
+  a.slots = p.slots;
+  a.slots_stride = p.slots_stride;
+  a.bounds = reinterpret_cast<uint16_t*>(p.key_bounds);
+  for (int i = 0; i < 3; ++i) a.bounds_stride[i] = p.bounds_stride[i];
+  a.num_tokens = p.num_tokens;
+  a.heads_kv = p.heads_kv;
+  a.num_blocks = p.num_blocks;
+  a.shift = log2_of(p.block_size);
+  // Tokens of a workgroup: one while the chip is not full of waves, then more,
+  // up to a block's worth, since most tokens of a long prompt lead no segment.
+  const int64_t waves = (int64_t)p.num_tokens * 2 * p.heads_kv;
+  a.chunk = 1;
+  while (a.chunk < p.block_size && a.chunk < 64 && waves / a.chunk > 16 * (int64_t)device_cu_count()) a.chunk *= 2;
+  return p.dtype == FA_DTYPE_F16 ? append_by_format<f16_t>(a, p.kv_format, p.head_dim, stream)
+                                 : append_by_format<bf16_t>(a, p.kv_format, p.head_dim, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Choice of blocks.  The score sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d is at
+// least q.k for every key within the bounds.  Sums are in 64 bits (products of
+// two 16-bit values are exact there), so that a block at the border does not
+// depend on the order of a sum; the vector units' rate for 64-bit FMAs hides
+// them behind the bounds' bytes.
+//
+// paged_score_kernel: a lane owns 4 dims of a block (D / 4 lanes a block, 64
+// at D = 512 with 8) and 4 query rows in registers; the 4 rows' sums are
+// folded over the lanes with the rows shared out, so that a step halves what
+// is left to add.  Each block's score goes to the workspace as an integer of
+// the same order.  paged_top_kernel: one workgroup per (sequence, KV head)
+// finds the n_index-th largest by 12-bit digits and writes the chosen ones in
+// index order.
+// ---------------------------------------------------------------------------
+namespace {
+constexpr int kScoreThreads = 256;
+constexpr int kScoreBlocks = 64;  // blocks of a workgroup
+constexpr int kScoreRows = 4;     // query rows at a time
+constexpr uint64_t kAlways = ~0ull;
+constexpr uint64_t kLowest = 0x000FFFFFFFFFFFFFull;  // order_of(-infinity)
+
+struct SelectArgs {
+  fa_select_params p;
+  uint64_t* keys;  // (batch, heads_kv, max_blocks)
+  int32_t shift;
+};
+
+// An integer that orders as the double does (NaN: as +infinity; -0 as 0).
+__device__ inline uint64_t order_of(double x) {
+  if (x != x) x = __builtin_inf();
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return (b >> 63) ? ~b : b | 0x8000000000000000ull;
+}
+
+__device__ inline int blocks_of(const SelectArgs& a, int b) {
+  const int64_t len = max(a.p.context_lens[b * a.p.context_lens_stride], 0);
+  return (int)min((int64_t)a.p.max_blocks, (len + a.p.block_size - 1) >> a.shift);
+}
+}  // namespace
+
+template <typename Tag, int D>
+__global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a) {
+  using EL = Elem<Tag>;
+  constexpr int LPB = D / 4 < 64 ? D / 4 : 64;  // lanes of a block
+  constexpr int DPL = D / LPB;                  // dims of a lane: 4, or 8 at D = 512
+  constexpr int BPW = 64 / LPB;                 // blocks a wave reads at a time
+  __shared__ uint64_t best[kScoreBlocks];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int n = blocks_of(a, b);
+  const int first = blockIdx.x * kScoreBlocks;
+  // A choice is only made among more than n_index blocks.
+  if (n <= a.p.n_index || first >= n) return;
+  const int group = a.p.heads_q / a.p.heads_kv, rows = group * a.p.seqlen_q;
+  const int c = lane % LPB, sub = lane / LPB;
+  const uint16_t* const bounds = reinterpret_cast<const uint16_t*>(a.p.key_bounds) + h * a.p.bounds_stride[1] + DPL * c;
+  constexpr int PER = kScoreBlocks / (kScoreThreads / 64) / BPW;  // passes of a wave over its blocks
+  for (int r0 = 0; r0 < rows; r0 += kScoreRows) {
+    double pos[kScoreRows][DPL], neg[kScoreRows][DPL];
+#pragma unroll
+    for (int r = 0; r < kScoreRows; ++r) {
+      const int row = min(r0 + r, rows - 1);  // (a row twice changes no maximum)
+      const int g = row / a.p.seqlen_q, m = row - g * a.p.seqlen_q;
+      const uint16_t* const q = reinterpret_cast<const uint16_t*>(a.p.q) + b * a.p.q_stride[0] +
+                                (h * group + g) * a.p.q_stride[1] + m * a.p.q_stride[2] + DPL * c;
+#pragma unroll
+      for (int e = 0; e < DPL; ++e) {
+        const float x = EL::to_f(q[e]);
+        pos[r][e] = x > 0.f ? (double)x : x == x ? 0.0 : (double)x;  // (NaN in both)
+        neg[r][e] = x < 0.f ? (double)x : x == x ? 0.0 : (double)x;
+      }
+    }
+    for (int i = 0; i < PER; ++i) {
+      const int k = (wave * PER + i) * BPW + sub;  // block of this lane, within the workgroup's
+      const int blk = min(first + k, n - 1);
+      const int page = a.p.block_table[b * a.p.block_table_stride[0] + blk * a.p.block_table_stride[1]];
+      const bool there = page >= 0 && page < a.p.num_blocks;
+      const uint16_t* const lo = bounds + (there ? page : 0) * a.p.bounds_stride[0];
+      const uint16_t* const hi = lo + a.p.bounds_stride[2];
+      double sum[kScoreRows] = {};
+#pragma unroll
+      for (int e0 = 0; e0 < DPL; e0 += 4) {
+        const s16x4 x = *reinterpret_cast<const s16x4*>(lo + e0), y = *reinterpret_cast<const s16x4*>(hi + e0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double l = EL::to_f((uint16_t)x[e]), u = EL::to_f((uint16_t)y[e]);
+#pragma unroll
+          for (int r = 0; r < kScoreRows; ++r) {
+            sum[r] = __builtin_fma(pos[r][e0 + e], u, sum[r]);
+            sum[r] = __builtin_fma(neg[r][e0 + e], l, sum[r]);
+          }
+        }
+      }
+      // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
+      const bool odd = lane & 1, two = lane & 2;
+      double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
+      u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
+      u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
+      double v = two ? u1 : u0;
+      v += __shfl_xor(two ? u0 : u1, 2, 64);
+#pragma unroll
+      for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
+      if (v != v) v = __builtin_inf();
+      v = fmax(v, __shfl_xor(v, 1, 64));
+      v = fmax(v, __shfl_xor(v, 2, 64));
+      if (c == 0) {
+        const uint64_t key = there ? order_of(v) : kLowest;
+        best[k] = r0 == 0 ? key : max(best[k], key);
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < kScoreBlocks && first + tid < n) {
+    const int blk = first + tid;
+    const bool always = blk < a.p.keep_first || blk >= n - a.p.keep_last;
+    a.keys[((int64_t)b * a.p.heads_kv + h) * a.p.max_blocks + blk] = always ? kAlways : best[tid];
+  }
+}
+
+namespace {
+constexpr int kTopThreads = 256;
+constexpr int kDigit = 12, kBins = 1 << kDigit;
+}  // namespace
+
+__global__ __launch_bounds__(kTopThreads) void paged_top_kernel(SelectArgs a) {
+  __shared__ uint32_t bins[kBins];
+  __shared__ uint32_t wave_sum[kTopThreads / 64];
+  __shared__ int32_t found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int n = blocks_of(a, b), want = a.p.n_index;
+  int32_t* const out = a.p.index + ((int64_t)b * a.p.heads_kv + h) * want;
+  if (n <= want) {
+    for (int i = tid; i < want; i += kTopThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const uint64_t* const keys = a.keys + ((int64_t)b * a.p.heads_kv + h) * a.p.max_blocks;
+  // The want-th largest key, digit by digit: `prefix` holds the digits found,
+  // `left` how many of the keys that share them are still to be taken.
+  uint64_t prefix = 0;
+  int left = want;
+  for (int top = 64; top > 0; top -= kDigit) {
+    const int low = max(top - kDigit, 0), width = top - low;
+    constexpr int PER = kBins / kTopThreads;
+    for (int i = tid; i < kBins; i += kTopThreads) bins[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kTopThreads) {
+      const uint64_t k = keys[i];
+      if (top == 64 || (k >> top) == (prefix >> top)) atomicAdd(&bins[(k >> low) & ((1u << width) - 1)], 1u);
+    }
+    __syncthreads();
+    // Thread t sums the bins [t * PER, (t + 1) * PER) from the highest thread down.
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += bins[tid * PER + i];
+    uint32_t above = mine;  // inclusive, over the lanes from this one up
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_down(above, o, 64);
+      if (lane + o < 64) above += y;
+    }
+    if (lane == 0) wave_sum[wave] = above;
+    __syncthreads();
+    above -= mine;
+    for (int w = wave + 1; w < kTopThreads / 64; ++w) above += wave_sum[w];
+    if ((int)above < left && (int)(above + mine) >= left) {
+      int digit = PER - 1;
+      uint32_t seen = above;
+      while ((int)(seen + bins[tid * PER + digit]) < left) seen += bins[tid * PER + digit--];
+      found[0] = tid * PER + digit;
+      found[1] = left - (int)seen;
+    }
+    __syncthreads();
+    prefix |= (uint64_t)found[0] << low;
+    left = found[1];
+    __syncthreads();
+  }
+  // Keys above `prefix`, and the first `left` equal to it, in index order.
+  int at = 0, equal = 0;
+  for (int i0 = 0; i0 < n; i0 += kTopThreads) {
+    const int i = i0 + tid;
+    const uint64_t k = i < n ? keys[i] : 0;
+    const uint64_t eq = __builtin_amdgcn_ballot_w64(i < n && k == prefix);
+    __syncthreads();
+    if (lane == 0) wave_sum[wave] = __builtin_popcountll(eq);
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+    int eq_before = equal + __builtin_popcountll(eq & below);
+    for (int w = 0; w < kTopThreads / 64; ++w) {
+      if (w < wave) eq_before += wave_sum[w];
+      equal += wave_sum[w];
+    }
+    const bool take = i < n && (k > prefix || (k == prefix && eq_before < left));
+    const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
+    __syncthreads();
+    if (lane == 0) wave_sum[wave] = __builtin_popcountll(tk);
+    __syncthreads();
+    int pos = at + __builtin_popcountll(tk & below);
+    for (int w = 0; w < kTopThreads / 64; ++w) {
+      if (w < wave) pos += wave_sum[w];
+      at += wave_sum[w];
+    }
+    if (take) out[pos] = i;
+  }
+}
+
+size_t select_workspace_bytes(int batch, int heads_kv, int max_blocks) {
+  return (size_t)batch * heads_kv * max_blocks * sizeof(uint64_t);
+}
+
+template <typename Tag>
+static hipError_t select_by_dim(const SelectArgs& a, hipStream_t stream) {
+  const dim3 grid((a.p.max_blocks + kScoreBlocks - 1) / kScoreBlocks, a.p.heads_kv, a.p.batch);
+  const dim3 block(kScoreThreads);
+  switch (a.p.head_dim) {
+    case 32: hipLaunchKernelGGL((paged_score_kernel<Tag, 32>), grid, block, 0, stream, a); break;
+    case 64: hipLaunchKernelGGL((paged_score_kernel<Tag, 64>), grid, block, 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((paged_score_kernel<Tag, 128>), grid, block, 0, stream, a); break;
+    case 256: hipLaunchKernelGGL((paged_score_kernel<Tag, 256>), grid, block, 0, stream, a); break;
+    case 512: hipLaunchKernelGGL((paged_score_kernel<Tag, 512>), grid, block, 0, stream, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_select(const fa_select_params& p, hipStream_t stream) {
+  SelectArgs a{};
+  a.p = p;
+  a.keys = reinterpret_cast<uint64_t*>(p.workspace);
+  a.shift = log2_of(p.block_size);
+  if (p.max_blocks > p.n_index) {
+    const hipError_t e = p.dtype == FA_DTYPE_F16 ? select_by_dim<f16_t>(a, stream) : select_by_dim<bf16_t>(a, stream);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(paged_top_kernel, dim3(p.heads_kv, p.batch), dim3(kTopThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace fa

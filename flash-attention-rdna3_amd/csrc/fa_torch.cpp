@@ -20,6 +20,9 @@
 //   decode(q, k, v, new_k?, new_v?, lens?, ...) -> out    split-K decode, after
 //             writing new_k / new_v into the cache when given
 //   decode_paged(q, k_cache, v_cache, block_table, context_lens, ...) -> out
+//   paged_allocate(block_table, context_lens, ...) -> (slots, cu_seqlens, next_head)
+//   paged_append(key, value, k_cache, v_cache, slots, ...)   in place
+//   paged_select(query, key_bounds, block_table, ...) -> index
 //   set_ds_scratch_limit(bytes) / ds_scratch_limit() -> bytes
 // Argument contracts are checked by the Python layer with the reference's
 // messages before any of these is called; the C ABI re-checks what could
@@ -565,6 +568,193 @@ Tensor decode_paged_op(const Tensor& query, const Tensor& k_cache, const Tensor&
   return kdim != head_dim ? out.narrow(-1, 0, head_dim) : out;
 }
 
+// ---------------------------------------------------------------------------
+// Filling a paged cache and choosing its blocks.  The Python layer has checked
+// the arguments with its messages; these check again what a kernel reads or
+// writes, since they may be called by themselves.
+// ---------------------------------------------------------------------------
+void abi_strides(int64_t* dst, const Tensor& t, bool unit_last = false) {
+  for (int64_t i = 0; i < t.dim(); ++i) dst[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  if (unit_last) dst[t.dim() - 1] = 1;
+}
+
+int32_t to_int32(int64_t n, const char* what) {
+  TORCH_CHECK(n >= 0 && n <= INT32_MAX, "fa_mi355x: ", what, " out of range: ", n);
+  return (int32_t)n;
+}
+
+// The tensor is written as it is: rows of 16-byte pieces, no copy.
+void check_in_place(const Tensor& t, const char* what) {
+  TORCH_CHECK(kernel_ready(t).is_same(t), "fa_mi355x: ", what, " needs a unit last stride and 16-byte aligned rows");
+}
+
+int kv_format_of(const Tensor& cache, const Tensor& like) {
+  if (cache.scalar_type() == at::kFloat8_e4m3fn) return FA_KV_E4M3;
+  if (cache.scalar_type() == at::kChar) return FA_KV_INT8;
+  TORCH_CHECK(cache.scalar_type() == like.scalar_type(),
+              "fa_mi355x: a cache must be float8_e4m3fn, int8 or of the query's dtype");
+  return FA_KV_SAME;
+}
+
+void check_16bit(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "fa_mi355x: ", what, " must be a GPU tensor");
+  TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, "fa_mi355x: ", what,
+              " must be float16 or bfloat16");
+}
+
+// Scales of an 8-bit cache (num_blocks, heads_kv, ...).
+void check_scales(const OptTensor& k_scale, const OptTensor& v_scale, const Tensor& cache) {
+  for (const OptTensor* t : {&k_scale, &v_scale})
+    TORCH_CHECK(t->has_value() && (*t)->device() == cache.device() && (*t)->scalar_type() == at::kFloat &&
+                    (*t)->dim() == 2 && (*t)->size(0) == cache.size(0) && (*t)->size(1) == cache.size(2),
+                "fa_mi355x: k_scale and v_scale must be float32 (num_blocks, heads_kv) on the cache's device");
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_allocate_op(const Tensor& block_table, const Tensor& context_lens,
+                                                     const Tensor& new_lens, const Tensor& free_blocks,
+                                                     const OptTensor& free_head, int64_t block_size,
+                                                     int64_t num_tokens) {
+  TORCH_CHECK(block_table.is_cuda() && block_table.dim() == 2, "fa_mi355x: block_table must be a 2-D GPU tensor");
+  const int64_t batch = block_table.size(0);
+  check_int32(block_table, block_table, block_table.sizes(), "block_table");
+  check_int32(context_lens, block_table, {batch}, "context_lens");
+  check_int32(new_lens, block_table, {batch}, "new_lens");
+  TORCH_CHECK(free_blocks.dim() == 1, "fa_mi355x: free_blocks must be 1-D");
+  check_int32(free_blocks, block_table, {free_blocks.size(0)}, "free_blocks");
+  if (free_head.has_value()) check_int32(*free_head, block_table, {1}, "free_head");
+  TORCH_CHECK(num_tokens >= 0, "fa_mi355x: num_tokens must not be negative");
+  c10::DeviceGuard guard(block_table.device());
+  const Tensor slots = at::empty({num_tokens}, block_table.options().dtype(at::kLong));
+  const Tensor cu = at::empty({batch + 1}, block_table.options()), next = at::empty({1}, block_table.options());
+  fa_allocate_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.abi_version = FA_ABI_VERSION;
+  p.batch = to_int32(batch, "batch");
+  p.block_table = block_table.data_ptr<int32_t>();
+  p.context_lens = context_lens.data_ptr<int32_t>();
+  p.new_lens = new_lens.data_ptr<int32_t>();
+  p.free_blocks = free_blocks.data_ptr<int32_t>();
+  p.free_head = free_head.has_value() ? free_head->data_ptr<int32_t>() : nullptr;
+  p.slots = slots.data_ptr<int64_t>();
+  p.cu_seqlens = cu.data_ptr<int32_t>();
+  p.next_head = next.data_ptr<int32_t>();
+  abi_strides(p.block_table_stride, block_table);
+  p.context_lens_stride = context_lens.stride(0);
+  p.new_lens_stride = new_lens.stride(0);
+  p.free_blocks_stride = free_blocks.stride(0);
+  p.max_blocks = to_int32(block_table.size(1), "blocks of a sequence");
+  p.block_size = to_int32(block_size, "block_size");
+  p.num_free = to_int32(free_blocks.size(0), "free_blocks");
+  p.num_tokens = to_int32(num_tokens, "num_tokens");
+  check_status(fa_paged_allocate(&p, stream_of(block_table)), "fa_paged_allocate");
+  return {slots, cu, next};
+}
+
+void paged_append_op(const Tensor& key, const Tensor& value, const Tensor& k_cache, const Tensor& v_cache,
+                     const Tensor& slots, const OptTensor& k_scale, const OptTensor& v_scale,
+                     const OptTensor& key_bounds) {
+  check_16bit(key, "key");
+  TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes() && value.scalar_type() == key.scalar_type() &&
+                  value.device() == key.device(),
+              "fa_mi355x: key and value must be (tokens, heads_kv, head_dim), of one dtype and device");
+  for (const Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->device() == key.device() && t->dim() == 4 && t->sizes() == k_cache.sizes() &&
+                    t->scalar_type() == k_cache.scalar_type() && t->size(2) == key.size(1) && t->size(3) == key.size(2),
+                "fa_mi355x: caches must be (blocks, block_size, heads_kv, head_dim) of one shape and dtype, on key's "
+                "device");
+  TORCH_CHECK(slots.device() == key.device() && slots.scalar_type() == at::kLong && slots.dim() == 1 &&
+                  slots.size(0) == key.size(0),
+              "fa_mi355x: slot_mapping must be int64 (tokens,) on key's device");
+  const int format = kv_format_of(k_cache, key);
+  if (format != FA_KV_SAME) check_scales(k_scale, v_scale, k_cache);
+  check_in_place(k_cache, "k_cache");
+  check_in_place(v_cache, "v_cache");
+  if (key_bounds.has_value()) {
+    TORCH_CHECK(key_bounds->device() == key.device() && key_bounds->scalar_type() == key.scalar_type() &&
+                    key_bounds->sizes() == at::IntArrayRef({k_cache.size(0), key.size(1), 2, key.size(2)}),
+                "fa_mi355x: key_bounds must be (blocks, heads_kv, 2, head_dim) in key's dtype, on its device");
+    check_in_place(*key_bounds, "key_bounds");
+  }
+  c10::DeviceGuard guard(key.device());
+  const Tensor kn = kernel_ready(key), vn = kernel_ready(value);
+  fa_paged_append_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.abi_version = FA_ABI_VERSION;
+  p.dtype = dtype_code(key.scalar_type());
+  p.k_new = kn.data_ptr();
+  p.v_new = vn.data_ptr();
+  p.k_cache = k_cache.data_ptr();
+  p.v_cache = v_cache.data_ptr();
+  p.slots = slots.data_ptr<int64_t>();
+  abi_strides(p.k_new_stride, kn, true);
+  abi_strides(p.v_new_stride, vn, true);
+  abi_strides(p.k_cache_stride, k_cache, true);
+  abi_strides(p.v_cache_stride, v_cache, true);
+  p.slots_stride = slots.stride(0);
+  if (format != FA_KV_SAME) {
+    p.k_scale = k_scale->data_ptr<float>();
+    p.v_scale = v_scale->data_ptr<float>();
+    abi_strides(p.k_scale_stride, *k_scale);
+    abi_strides(p.v_scale_stride, *v_scale);
+  }
+  if (key_bounds.has_value()) {
+    p.key_bounds = key_bounds->data_ptr();
+    abi_strides(p.bounds_stride, *key_bounds, true);
+  }
+  p.num_tokens = to_int32(key.size(0), "tokens");
+  p.heads_kv = to_int32(key.size(1), "heads_kv");
+  p.head_dim = to_int32(key.size(2), "head_dim");
+  p.num_blocks = to_int32(k_cache.size(0), "blocks");
+  p.block_size = to_int32(k_cache.size(1), "block_size");
+  p.kv_format = format;
+  check_status(fa_paged_append(&p, stream_of(key)), "fa_paged_append");
+}
+
+Tensor paged_select_op(const Tensor& query, const Tensor& key_bounds, const Tensor& block_table,
+                       const Tensor& context_lens, int64_t num_selected, int64_t block_size, int64_t keep_first,
+                       int64_t keep_last) {
+  check_16bit(query, "query");
+  TORCH_CHECK(query.dim() == 4, "fa_mi355x: query must be (batch, heads, rows, head_dim)");
+  TORCH_CHECK(key_bounds.device() == query.device() && key_bounds.scalar_type() == query.scalar_type() &&
+                  key_bounds.dim() == 4 && key_bounds.size(2) == 2 && key_bounds.size(3) == query.size(3),
+              "fa_mi355x: key_bounds must be (blocks, heads_kv, 2, head_dim) in the query's dtype, on its device");
+  TORCH_CHECK(block_table.dim() == 2, "fa_mi355x: block_table must be 2-D");
+  check_int32(block_table, query, {query.size(0), block_table.size(1)}, "block_table");
+  check_int32(context_lens, query, {query.size(0)}, "context_lens");
+  c10::DeviceGuard guard(query.device());
+  const Tensor q = kernel_ready(query), bounds = kernel_ready(key_bounds);
+  fa_select_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.n_index = to_int32(num_selected, "num_selected");
+  p.batch = to_int32(q.size(0), "batch");
+  p.heads_kv = to_int32(bounds.size(1), "heads_kv");
+  p.max_blocks = to_int32(block_table.size(1), "blocks of a sequence");
+  const Tensor index = at::empty({q.size(0), bounds.size(1), num_selected}, query.options().dtype(at::kInt));
+  const size_t bytes = fa_select_workspace_bytes(p.batch, p.heads_kv, p.max_blocks);
+  const Tensor ws = at::empty({(int64_t)bytes}, query.options().dtype(at::kByte));
+  p.abi_version = FA_ABI_VERSION;
+  p.dtype = dtype_code(q.scalar_type());
+  p.q = q.data_ptr();
+  p.key_bounds = bounds.data_ptr();
+  p.block_table = block_table.data_ptr<int32_t>();
+  p.context_lens = context_lens.data_ptr<int32_t>();
+  p.index = index.data_ptr<int32_t>();
+  abi_strides(p.q_stride, q, true);
+  abi_strides(p.bounds_stride, bounds, true);
+  abi_strides(p.block_table_stride, block_table);
+  p.context_lens_stride = context_lens.stride(0);
+  p.heads_q = to_int32(q.size(1), "heads");
+  p.seqlen_q = to_int32(q.size(2), "rows");
+  p.head_dim = to_int32(q.size(3), "head_dim");
+  p.num_blocks = to_int32(bounds.size(0), "blocks");
+  p.block_size = to_int32(block_size, "block_size");
+  p.keep_first = to_int32(keep_first, "keep_first");
+  p.keep_last = to_int32(keep_last, "keep_last");
+  p.workspace = ws.data_ptr();
+  check_status(fa_paged_select(&p, stream_of(query)), "fa_paged_select");
+  return index;
+}
+
 // Inside a torch.func transform.  Decode has no rule for any of them, and a
 // wrapped argument must not reach it: a jvp would come back with a silent zero
 // tangent.  Plain tensors are not the transform's business.
@@ -585,6 +775,9 @@ int64_t set_ds_scratch_limit(int64_t bytes) {
 
 int64_t ds_scratch_limit() { return g_ds_limit.load(); }
 
+// Operators that stay outside autograd and torch.func.
+constexpr const char* kInferenceOnly[] = {"decode", "decode_paged", "paged_allocate", "paged_append", "paged_select"};
+
 }  // namespace
 
 TORCH_LIBRARY(fa_mi355x, m) {
@@ -599,6 +792,12 @@ TORCH_LIBRARY(fa_mi355x, m) {
         "float scale, int num_splits, bool kv_fp8, float k_scale, float v_scale, Tensor(c!)? tickets) -> Tensor");
   m.def("decode_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, bool causal, "
         "float scale, int num_splits, bool kv_fp8, float k_scale, float v_scale, Tensor(a!)? tickets) -> Tensor");
+  m.def("paged_allocate(Tensor(a!) block_table, Tensor context_lens, Tensor new_lens, Tensor free_blocks, "
+        "Tensor? free_head, int block_size, int num_tokens) -> (Tensor, Tensor, Tensor)");
+  m.def("paged_append(Tensor key, Tensor value, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slot_mapping, "
+        "Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(e!)? key_bounds) -> ()");
+  m.def("paged_select(Tensor query, Tensor key_bounds, Tensor block_table, Tensor context_lens, int num_selected, "
+        "int block_size, int keep_first, int keep_last) -> Tensor");
   m.def("set_ds_scratch_limit(int bytes) -> int", &set_ds_scratch_limit);
   m.def("ds_scratch_limit() -> int", &ds_scratch_limit);
 }
@@ -610,6 +809,9 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
   m.impl("backward", &backward_op);
   m.impl("decode", &decode_op);
   m.impl("decode_paged", &decode_paged_op);
+  m.impl("paged_allocate", &paged_allocate_op);
+  m.impl("paged_append", &paged_append_op);
+  m.impl("paged_select", &paged_select_op);
 }
 
 // Decode is inference-only: like a launch on raw pointers, its output and the
@@ -619,18 +821,16 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
 // as requiring grad, and its version counters would refuse caches made in
 // inference mode.
 TORCH_LIBRARY_IMPL(fa_mi355x, Autograd, m) {
-  m.impl("decode", torch::CppFunction::makeFallthrough());
-  m.impl("decode_paged", torch::CppFunction::makeFallthrough());
+  for (const char* name : kInferenceOnly) m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(fa_mi355x, FuncTorchDynamicLayerFrontMode, m) {
-  m.impl("decode", torch::CppFunction::makeFromBoxedFunction<&decode_in_transform>());
-  m.impl("decode_paged", torch::CppFunction::makeFromBoxedFunction<&decode_in_transform>());
+  for (const char* name : kInferenceOnly)
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&decode_in_transform>());
 }
 
 TORCH_LIBRARY_IMPL(fa_mi355x, ADInplaceOrView, m) {
-  m.impl("decode", torch::CppFunction::makeFallthrough());
-  m.impl("decode_paged", torch::CppFunction::makeFallthrough());
+  for (const char* name : kInferenceOnly) m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 TORCH_LIBRARY_IMPL(fa_mi355x, Meta, m) {

@@ -14,6 +14,11 @@ from .interface import (
     flash_attention_with_kvcache,
     alibi_slopes,
 )
+from .paged import (
+    paged_kvcache_allocate,
+    paged_kvcache_append,
+    paged_kvcache_select,
+)
 from .sdpa import (
     disable_rdna3_flash_attention,
     enable_rdna3_flash_attention,
@@ -27,6 +32,9 @@ __all__ = [
     "flash_attention_decode_paged",
     "flash_attention_decode_paged_multi",
     "flash_attention_with_kvcache",
+    "paged_kvcache_allocate",
+    "paged_kvcache_append",
+    "paged_kvcache_select",
     "alibi_slopes",
     "is_available",
     "unsupported_reason",

@@ -121,13 +121,75 @@ class TinyParams(ctypes.Structure):
     ]
 
 
-_STRUCTS = (FwdParams, BwdParams, DecodeParams, PagedParams, TinyParams, AppendParams)
+class PagedBlocksParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("context_lens", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("block_index", ctypes.c_void_p),
+        ("q_stride", _i64_4), ("k_stride", _i64_4), ("v_stride", _i64_4), ("out_stride", _i64_4),
+        ("block_table_stride", _i64_2), ("context_lens_stride", ctypes.c_int64),
+        ("k_scale_stride", _i64_2), ("v_scale_stride", _i64_2), ("block_index_stride", _i64_3),
+        ("batch", ctypes.c_int32), ("heads_q", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("num_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32), ("n_index", ctypes.c_int32), ("seqlen_q", ctypes.c_int32),
+        ("kv_format", ctypes.c_int32), ("softmax_scale", ctypes.c_float), ("causal", ctypes.c_int32),
+        ("shares", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("tickets", ctypes.c_void_p),
+    ]
+
+
+class AllocateParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("batch", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p), ("context_lens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p), ("free_head", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("cu_seqlens", ctypes.c_void_p), ("next_head", ctypes.c_void_p),
+        ("block_table_stride", _i64_2), ("context_lens_stride", ctypes.c_int64),
+        ("new_lens_stride", ctypes.c_int64), ("free_blocks_stride", ctypes.c_int64),
+        ("max_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("num_free", ctypes.c_int32), ("num_tokens", ctypes.c_int32),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("key_bounds", ctypes.c_void_p),
+        ("k_new_stride", _i64_3), ("v_new_stride", _i64_3),
+        ("k_cache_stride", _i64_4), ("v_cache_stride", _i64_4), ("slots_stride", ctypes.c_int64),
+        ("k_scale_stride", _i64_2), ("v_scale_stride", _i64_2), ("bounds_stride", _i64_4),
+        ("num_tokens", ctypes.c_int32), ("heads_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32), ("block_size", ctypes.c_int32), ("kv_format", ctypes.c_int32),
+    ]
+
+
+class SelectParams(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("key_bounds", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p), ("index", ctypes.c_void_p),
+        ("q_stride", _i64_4), ("bounds_stride", _i64_4), ("block_table_stride", _i64_2),
+        ("context_lens_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("heads_q", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("seqlen_q", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32), ("max_blocks", ctypes.c_int32), ("n_index", ctypes.c_int32),
+        ("keep_first", ctypes.c_int32), ("keep_last", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+    ]
+
+
+_STRUCTS = (FwdParams, BwdParams, DecodeParams, PagedParams, TinyParams, AppendParams, PagedBlocksParams,
+            AllocateParams, PagedAppendParams, SelectParams)
 EXPORTS = (
     "fa_abi_version", "fa_last_error_string", "fa_params_size", "fa_decode_workspace_bytes",
     "fa_decode_ticket_count",
     "fa_fwd", "fa_fwd_ws", "fa_fwd_workspace_bytes", "fa_bwd", "fa_bwd_phase", "fa_bwd_workspace_bytes", "fa_bwd_workspace_min_bytes", "fa_decode_splitk", "fa_decode_splitk_noalloc", "fa_decode_paged",
     "fa_tiny_fwd_f32",
     "fa_kvcache_append",
+    "fa_paged_allocate", "fa_paged_append", "fa_paged_select", "fa_select_workspace_bytes",
     "fa_hbm_read_probe_count", "fa_hbm_read_probe_name", "fa_hbm_read_probe",
 )
 
@@ -172,10 +234,14 @@ def lib():
         for name, struct in (("fa_fwd", FwdParams), ("fa_bwd", BwdParams),
                              ("fa_decode_splitk", DecodeParams), ("fa_decode_splitk_noalloc", DecodeParams),
                              ("fa_decode_paged", PagedParams),
-                             ("fa_tiny_fwd_f32", TinyParams), ("fa_kvcache_append", AppendParams)):
+                             ("fa_tiny_fwd_f32", TinyParams), ("fa_kvcache_append", AppendParams),
+                             ("fa_paged_allocate", AllocateParams), ("fa_paged_append", PagedAppendParams),
+                             ("fa_paged_select", SelectParams)):
             fn = getattr(handle, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+        handle.fa_select_workspace_bytes.restype = ctypes.c_size_t
+        handle.fa_select_workspace_bytes.argtypes = [ctypes.c_int] * 3
         handle.fa_bwd_phase.restype = ctypes.c_int
         handle.fa_hbm_read_probe_count.restype = ctypes.c_int
         handle.fa_hbm_read_probe_name.restype = ctypes.c_char_p

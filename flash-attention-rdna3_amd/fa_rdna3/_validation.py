@@ -214,3 +214,120 @@ def validate_paged_inputs(query, key, value, block_table, context_lens):
     if block_table.shape[1] <= 0:
         raise ValueError("block_table must contain at least one logical block")
     _require_platform(query.device)
+
+
+# ---------------------------------------------------------------------------
+# Filling a paged cache and choosing its blocks (paged.py)
+# ---------------------------------------------------------------------------
+
+EIGHT_BIT_DTYPES = (torch.float8_e4m3fn, torch.int8)
+EIGHT_BIT_HEAD_DIMS = (32, 64, 128, 256, 512)
+
+
+def _require_count(name, value, least):
+    if isinstance(value, bool) or not isinstance(value, Integral) or not least <= value < 2 ** 31:
+        raise ValueError(f"{name} must be an integer of at least {least}")
+
+
+def _require_block_size(block_size):
+    _require_count("block_size", block_size, 1)
+    if block_size > 256 or block_size & (block_size - 1):
+        raise ValueError("paged cache block size must be a power of two up to 256")
+
+
+def _require_like(name, tensor, dtype, shape, device):
+    """A tensor of this dtype, shape (None: any extent) and device."""
+    _require_tensor(name, tensor)
+    if (tensor.device != device or tensor.dtype != dtype or tensor.dim() != len(shape)
+            or any(want is not None and got != want for got, want in zip(tensor.shape, shape))):
+        want = ", ".join("n" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be a {str(dtype).removeprefix('torch.')} tensor of shape ({want}) on {device}")
+
+
+def _require_writable(name, tensor, rows=False):
+    """A tensor that a kernel can write in place: no element twice and, for
+    `rows`, 16-byte pieces."""
+    if any(n > 1 and st == 0 for n, st in zip(tensor.shape, tensor.stride())):
+        raise ValueError(f"{name} is written in place and must not be expanded")
+    esize = tensor.element_size()
+    if rows and (tensor.stride(-1) != 1 or tensor.data_ptr() % 16
+                 or any(n > 1 and (st * esize) % 16 for st, n in zip(tensor.stride()[:-1], tensor.shape[:-1]))):
+        raise ValueError(f"{name} must have a unit last stride and 16-byte aligned rows to be updated in place")
+
+
+def validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, free_head, block_size, num_tokens):
+    _require_tensor("block_table", block_table)
+    device = block_table.device
+    _require_like("block_table", block_table, torch.int32, (None, None), device)
+    batch, blocks = block_table.shape
+    if batch <= 0 or blocks <= 0:
+        raise ValueError("block_table must have at least one sequence and one block")
+    _require_like("context_lens", context_lens, torch.int32, (batch,), device)
+    _require_like("new_lens", new_lens, torch.int32, (batch,), device)
+    _require_like("free_blocks", free_blocks, torch.int32, (None,), device)
+    if free_head is not None:
+        _require_like("free_head", free_head, torch.int32, (1,), device)
+    _require_block_size(block_size)
+    _require_count("num_tokens", num_tokens, 0)
+    _require_writable("block_table", block_table)
+    _require_platform(device)
+
+
+def validate_append_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, key_bounds):
+    _require_tensor("key", key)
+    device = key.device
+    if key.dim() != 3 or key.dtype not in LOW_PRECISION_DTYPES:
+        raise ValueError("key must be a float16 or bfloat16 tensor of shape (tokens, kv_heads, head_dim)")
+    tokens, heads, dim = key.shape
+    _require_like("value", value, key.dtype, (tokens, heads, dim), device)
+    _require_tensor("k_cache", k_cache)
+    if k_cache.dtype != key.dtype and k_cache.dtype not in EIGHT_BIT_DTYPES:
+        raise ValueError("caches must have key's dtype, float8_e4m3fn or int8")
+    _require_like("k_cache", k_cache, k_cache.dtype, (None, None, heads, dim), device)
+    _require_like("v_cache", v_cache, k_cache.dtype, k_cache.shape, device)
+    if min(heads, dim, k_cache.shape[0]) <= 0:
+        raise ValueError("kv_heads, head_dim and blocks must be positive")
+    _require_block_size(k_cache.shape[1])
+    eight = k_cache.dtype in EIGHT_BIT_DTYPES
+    if dim not in (EIGHT_BIT_HEAD_DIMS if eight else SUPPORTED_HEAD_DIMS):
+        raise ValueError(f"head_dim {dim} is not supported by a paged cache of {str(k_cache.dtype).removeprefix('torch.')}")
+    _require_like("slot_mapping", slot_mapping, torch.int64, (tokens,), device)
+    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if eight:
+            _require_like(name, scale, torch.float32, (k_cache.shape[0], heads), device)
+            _require_writable(name, scale)
+        elif scale is not None:
+            raise ValueError("k_scale and v_scale apply to float8_e4m3fn and int8 caches only")
+    _require_writable("k_cache", k_cache, rows=True)
+    _require_writable("v_cache", v_cache, rows=True)
+    if key_bounds is not None:
+        _require_like("key_bounds", key_bounds, key.dtype, (k_cache.shape[0], heads, 2, dim), device)
+        _require_writable("key_bounds", key_bounds, rows=True)
+    _require_platform(device)
+
+
+def validate_select_inputs(query, key_bounds, block_table, context_lens, num_selected, block_size, keep_first,
+                           keep_last):
+    _require_tensor("query", query)
+    device = query.device
+    if query.dim() not in (3, 4) or query.dtype not in LOW_PRECISION_DTYPES:
+        raise ValueError("query must be a float16 or bfloat16 tensor (batch, q_heads[, rows], head_dim)")
+    batch, heads, dim = query.shape[0], query.shape[1], query.shape[-1]
+    _require_like("key_bounds", key_bounds, query.dtype, (None, None, 2, dim), device)
+    if min(query.shape) <= 0 or min(key_bounds.shape) <= 0:
+        raise ValueError("batch, heads, rows, blocks and head_dim must be positive")
+    if dim not in EIGHT_BIT_HEAD_DIMS:
+        raise ValueError(f"head_dim {dim} is not supported by block selection")
+    if heads % key_bounds.shape[1]:
+        raise ValueError("query heads must be a multiple of cache heads")
+    _require_like("block_table", block_table, torch.int32, (batch, None), device)
+    if block_table.shape[1] <= 0:
+        raise ValueError("block_table must contain at least one logical block")
+    _require_like("context_lens", context_lens, torch.int32, (batch,), device)
+    _require_block_size(block_size)
+    _require_count("num_selected", num_selected, 1)
+    _require_count("keep_first", keep_first, 0)
+    _require_count("keep_last", keep_last, 0)
+    if keep_first + keep_last > num_selected:
+        raise ValueError("keep_first + keep_last must not exceed num_selected")
+    _require_platform(device)

@@ -297,6 +297,177 @@ typedef struct fa_tiny_params {
   int32_t reserved0;
 } fa_tiny_params;
 
+/*
+ * Paged decode over 8-bit caches with a scale for each block and head, and
+ * over selected blocks (no counterpart in the reference).
+ *
+ * Shapes, context_lens, block_table and causal are as in fa_paged_params.  Key n of a sequence is
+ * K = code * k_scale[page][head] (V likewise).  With block_index, KV head h
+ * of sequence b attends the logical blocks block_index[b][h][0..n_index) in
+ * place of all of them: an entry outside [0, ceil(context / block_size)) is
+ * no block, and one that is listed twice counts twice.  Keys keep the
+ * positions of their logical blocks, so `causal` means the same as without.
+ */
+typedef enum fa_kv_format {
+  FA_KV_SAME = 0, /* 16-bit, the query's type; scales NULL */
+  FA_KV_E4M3 = 1, /* fp8 (OCP e4m3) */
+  FA_KV_INT8 = 2
+} fa_kv_format;
+
+typedef struct fa_paged_blocks_params {
+  int32_t abi_version;
+  int32_t dtype; /* FA_DTYPE_F16 or FA_DTYPE_BF16: q and out */
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  const float* k_scale; /* (num_blocks, heads_kv); NULL: 1 */
+  const float* v_scale;
+  const int32_t* block_index; /* NULL: every block; else (batch, heads_kv, n_index) */
+  int64_t q_stride[4];        /* batch, head, row, dim */
+  int64_t k_stride[4];        /* block, position, head, dim */
+  int64_t v_stride[4];
+  int64_t out_stride[4];
+  int64_t block_table_stride[2];
+  int64_t context_lens_stride;
+  int64_t k_scale_stride[2];
+  int64_t v_scale_stride[2];
+  int64_t block_index_stride[3];
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim; /* 32, 64, 128, 256 or 512 */
+  int32_t num_blocks;
+  int32_t block_size; /* power of two, 1..256 */
+  int32_t max_blocks;
+  int32_t n_index;
+  int32_t seqlen_q;
+  int32_t kv_format; /* fa_kv_format */
+  float softmax_scale;
+  int32_t causal;
+  int32_t shares;    /* workgroups that share the keys of one (KV head, row block); 1..4096 */
+  int32_t reserved0;
+  void* workspace;   /* fa_paged_blocks_workspace_bytes(params) bytes, 16-byte aligned */
+  uint32_t* tickets; /* NULL: the shares are merged by a second launch; else
+                        fa_decode_ticket_count(batch, heads_q, seqlen_q) counters,
+                        zero before the call and left zero by it */
+} fa_paged_blocks_params;
+
+/*
+ * Block tables and slot maps from request lengths (no counterpart in the
+ * reference, whose paged decode takes ready tables).  Sequence b has
+ * max(context_lens[b], 0) cached tokens and gets max(new_lens[b], 0) more.
+ * Blocks it lacks for them are free_blocks[head], free_blocks[head + 1], ...
+ * in the order of the sequences (head = max(*free_head, 0), 0 for NULL), are
+ * entered into block_table, and each new token's slot is
+ * page * block_size + position in the page.  Past the end of free_blocks the
+ * entries are -1, and so are the slots of tokens without a page, of tokens
+ * past max_blocks * block_size and of rows past the last token.
+ * cu_seqlens (batch + 1) are the running sums of the new lengths; next_head is
+ * head plus the blocks that were asked for.
+ */
+typedef struct fa_allocate_params {
+  int32_t abi_version;
+  int32_t batch;
+  int32_t* block_table; /* (batch, max_blocks), new entries written in place */
+  const int32_t* context_lens;
+  const int32_t* new_lens;
+  const int32_t* free_blocks;
+  const int32_t* free_head; /* NULL: 0 */
+  int64_t* slots;           /* (num_tokens), contiguous */
+  int32_t* cu_seqlens;      /* (batch + 1), contiguous */
+  int32_t* next_head;       /* (1) */
+  int64_t block_table_stride[2];
+  int64_t context_lens_stride;
+  int64_t new_lens_stride;
+  int64_t free_blocks_stride;
+  int32_t max_blocks;
+  int32_t block_size; /* power of two, 1..256 */
+  int32_t num_free;
+  int32_t num_tokens;
+} fa_allocate_params;
+
+/*
+ * Appends rows to a paged cache in place (no counterpart in the reference).
+ * Token t goes to slot slots[t] = page * block_size + position; a slot outside
+ * the cache drops its row.  The tokens of one block have different slots and
+ * lie within block_size consecutive rows, with none of another block between
+ * them; rows of the block below the lowest of them are valid rows of before,
+ * and a block whose position 0 is written starts afresh.
+ * 8-bit caches: scale[page][head] becomes the larger of the scale of before
+ * (valid rows only) and the least power of two 2^e, e >= -100, with
+ * |x| <= top * 2^e for the new finite values (top 448 or 127); valid rows are
+ * rounded again where the scale grew.  Values are rounded to nearest, ties to
+ * even; infinities are stored as +-top, NaN as NaN (int8: 0).
+ * key_bounds, when not NULL: per page, head and dim the least and the greatest
+ * new or valid key (16-bit values as given; NaN left out).
+ */
+typedef struct fa_paged_append_params {
+  int32_t abi_version;
+  int32_t dtype; /* FA_DTYPE_F16 or FA_DTYPE_BF16: k_new, v_new, key_bounds */
+  const void* k_new;
+  const void* v_new;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slots;
+  float* k_scale; /* 8-bit caches: (num_blocks, heads_kv) */
+  float* v_scale;
+  void* key_bounds;       /* NULL, or (num_blocks, heads_kv, 2, head_dim) */
+  int64_t k_new_stride[3]; /* token, head, dim */
+  int64_t v_new_stride[3];
+  int64_t k_cache_stride[4]; /* block, position, head, dim */
+  int64_t v_cache_stride[4];
+  int64_t slots_stride;
+  int64_t k_scale_stride[2];
+  int64_t v_scale_stride[2];
+  int64_t bounds_stride[4];
+  int32_t num_tokens;
+  int32_t heads_kv;
+  int32_t head_dim; /* 16 (16-bit caches), 32, 64, 128, 256 or 512 */
+  int32_t num_blocks;
+  int32_t block_size; /* power of two, 1..256 */
+  int32_t kv_format;  /* fa_kv_format */
+} fa_paged_append_params;
+
+/*
+ * The blocks of each sequence and KV head whose key bounds allow the highest
+ * logits (no counterpart in the reference).  The score of a block is the
+ * greatest over the head group's query rows of
+ * sum_d max(q_d, 0) * hi_d + min(q_d, 0) * lo_d, summed in 64 bits; NaN counts
+ * as +infinity.  The first keep_first and the last keep_last blocks of a
+ * sequence are always in, then the highest scores (equal ones: the lowest
+ * index).  `index` gets the chosen logical blocks in ascending order and -1
+ * behind them.  A block whose table entry is no page scores -infinity.
+ */
+typedef struct fa_select_params {
+  int32_t abi_version;
+  int32_t dtype; /* FA_DTYPE_F16 or FA_DTYPE_BF16: q, key_bounds */
+  const void* q;          /* (batch, heads_q, seqlen_q, head_dim) */
+  const void* key_bounds; /* (num_blocks, heads_kv, 2, head_dim) */
+  const int32_t* block_table;
+  const int32_t* context_lens;
+  int32_t* index; /* (batch, heads_kv, n_index), contiguous */
+  int64_t q_stride[4];
+  int64_t bounds_stride[4];
+  int64_t block_table_stride[2];
+  int64_t context_lens_stride;
+  int32_t batch;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t seqlen_q;
+  int32_t head_dim; /* 32, 64, 128, 256 or 512 */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t max_blocks;
+  int32_t n_index;
+  int32_t keep_first;
+  int32_t keep_last;
+  int32_t reserved0;
+  void* workspace; /* fa_select_workspace_bytes(batch, heads_kv, max_blocks), 16-byte aligned */
+} fa_select_params;
+
 /* Version of this header the library was built from (FA_ABI_VERSION). */
 int fa_abi_version(void);
 
@@ -305,7 +476,7 @@ const char* fa_last_error_string(void);
 
 /* sizeof() of each params struct as compiled into the library, so a binding
  * can verify its own layout: which = 0 fwd, 1 bwd, 2 decode, 3 paged, 4 tiny,
- * 5 append. */
+ * 5 append, 6 paged blocks, 7 allocate, 8 paged append, 9 select. */
 size_t fa_params_size(int which);
 
 /* Bytes of scratch the split-K and paged decode need for `num_splits`. */
@@ -383,6 +554,10 @@ int fa_decode_splitk(const fa_decode_params* params, void* stream);
 #define FA_NOALLOC_TICKETS 65536
 int fa_decode_splitk_noalloc(const fa_decode_params* params, void* stream);
 int fa_decode_paged(const fa_paged_params* params, void* stream);
+int fa_paged_allocate(const fa_allocate_params* params, void* stream);
+int fa_paged_append(const fa_paged_append_params* params, void* stream);
+size_t fa_select_workspace_bytes(int batch, int heads_kv, int max_blocks);
+int fa_paged_select(const fa_select_params* params, void* stream);
 
 /*
  * HBM streaming-read probe.  No counterpart in the reference: it is the
