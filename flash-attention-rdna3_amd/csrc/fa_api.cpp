@@ -349,6 +349,52 @@ bool grid_ok(int64_t n) { return n <= 65535; }
 
 }  // namespace
 
+// Shape and type checks that the scratch size needs as well.
+static int check_paged_blocks(const fa_paged_blocks_params* params) {
+  if (!params) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: params is NULL");
+  const fa_paged_blocks_params& p = *params;
+  if (p.abi_version != FA_ABI_VERSION) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: abi_version mismatch");
+  if (p.dtype != FA_DTYPE_F16 && p.dtype != FA_DTYPE_BF16)
+    return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: dtype must be f16 or bf16");
+  if (p.kv_format < FA_KV_SAME || p.kv_format > FA_KV_INT8)
+    return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: kv_format %d", p.kv_format);
+  if (!dim_ok(p.head_dim)) return fail(FA_ERR_UNSUPPORTED, "fa_decode_paged_blocks: head_dim %d", p.head_dim);
+  if (p.batch <= 0 || p.heads_q <= 0 || p.heads_kv <= 0 || p.heads_q % p.heads_kv || p.seqlen_q <= 0 ||
+      p.num_blocks <= 0 || p.max_blocks <= 0 || !block_size_ok(p.block_size) || !grid_ok(p.batch) ||
+      (int64_t)p.heads_q * p.seqlen_q > INT32_MAX)
+    return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: bad shape");
+  if (p.shares < 0 || p.shares > 4096) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: shares must lie in 0..4096");
+  // Positions and the running count of 32-key chunks are 32-bit numbers.
+  const int64_t keys = (int64_t)std::max(p.max_blocks, p.block_index ? p.n_index : 0) * p.block_size;
+  if (keys > (int64_t(1) << 30) || p.batch * (keys / 32 + 1) > INT32_MAX)
+    return fail(FA_ERR_UNSUPPORTED, "fa_decode_paged_blocks: block tables of %lld keys for %d sequences", (long long)keys, p.batch);
+  return FA_OK;
+}
+
+size_t fa_paged_blocks_workspace_bytes(const fa_paged_blocks_params* params) {
+  return check_paged_blocks(params) == FA_OK ? fa::paged_blocks_workspace_bytes(*params) : 0;
+}
+
+int fa_decode_paged_blocks(const fa_paged_blocks_params* params, void* stream) {
+  const int rc = check_paged_blocks(params);
+  if (rc != FA_OK) return rc;
+  const fa_paged_blocks_params& p = *params;
+  if (p.causal != 0 && p.causal != 1) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: causal must be 0 or 1");
+  const int kes = p.kv_format == FA_KV_SAME ? 2 : 1;
+  if (!rows_ok(p.q, p.q_stride, 4, 2) || !rows_ok(p.k_cache, p.k_stride, 4, kes) ||
+      !rows_ok(p.v_cache, p.v_stride, 4, kes) || !rows_ok(p.out, p.out_stride, 4, 2))
+    return fail(FA_ERR_INVALID,
+                "fa_decode_paged_blocks: q/caches/out need a unit last stride and 16-byte aligned rows");
+  if (!p.block_table || !p.context_lens) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: metadata is NULL");
+  if (p.kv_format == FA_KV_SAME && (p.k_scale || p.v_scale))
+    return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: scales are for 8-bit caches");
+  if (p.block_index && p.n_index <= 0) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: n_index");
+  if (!p.workspace || !aligned16(p.workspace)) return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: workspace");
+  if ((reinterpret_cast<uintptr_t>(p.tickets) & 3u) != 0)
+    return fail(FA_ERR_INVALID, "fa_decode_paged_blocks: tickets");
+  return from_hip(fa::launch_paged_blocks(p, (hipStream_t)stream), "fa_decode_paged_blocks");
+}
+
 int fa_paged_allocate(const fa_allocate_params* params, void* stream) {
   if (!params) return fail(FA_ERR_INVALID, "fa_paged_allocate: params is NULL");
   const fa_allocate_params& p = *params;

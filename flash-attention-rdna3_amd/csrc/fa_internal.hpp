@@ -44,6 +44,8 @@ hipError_t launch_append(const fa_append_params& p, hipStream_t stream);
 hipError_t launch_allocate(const fa_allocate_params& p, hipStream_t stream);
 hipError_t launch_paged_append(const fa_paged_append_params& p, hipStream_t stream);
 hipError_t launch_select(const fa_select_params& p, hipStream_t stream);
+hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t stream);
+size_t paged_blocks_workspace_bytes(const fa_paged_blocks_params& p);
 size_t select_workspace_bytes(int batch, int heads_kv, int max_blocks);
 
 size_t decode_workspace_bytes(int batch, int heads_q, int seqlen_q, int head_dim, int num_splits);

@@ -1,0 +1,144 @@
+// fa_paged_attn.hip - launches of the paged attention over block scales and
+// listed blocks (fa_paged_attn.hpp).
+#include "fa_paged_attn.hpp"
+
+namespace fa {
+
+namespace {
+
+int log2_floor(int n) {
+  int s = 0;
+  while ((2 << s) <= n) ++s;
+  return s;
+}
+
+// Row blocks of 16 that a wave holds (R): more of them share the conversion
+// and the loads of a chunk.
+int row_blocks(const fa_paged_blocks_params& p) {
+  const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
+  if (p.kv_format == FA_KV_SAME || p.head_dim > 128 || p.block_size < 16 || rows <= 16) return 1;
+  return rows <= 32 ? 2 : 4;
+}
+
+struct Plan {
+  int r, head_shift, nrb, rb_rows, shares;
+};
+
+Plan plan_of(const fa_paged_blocks_params& p) {
+  Plan w;
+  w.r = row_blocks(p);
+  const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
+  w.nrb = (int)((rows + 16 * w.r - 1) / (16 * w.r));
+  w.rb_rows = (int)std::min<int64_t>(rows, 16 * w.r);
+  w.head_shift = 0;
+#ifdef FA_HEAD_SHIFT
+  w.head_shift = std::min(FA_HEAD_SHIFT, log2_floor(p.heads_kv & -p.heads_kv));
+#endif
+  const int64_t columns = (int64_t)(p.heads_kv >> w.head_shift) * w.nrb;
+  w.shares = p.shares > 0 ? p.shares
+                          : (int)std::max<int64_t>(1, (device_cu_count() + columns - 1) / columns);
+  return w;
+}
+
+int64_t partial_rows(const fa_paged_blocks_params& p, const Plan& w) {
+  return 2 * (int64_t)w.shares * p.heads_kv * w.nrb * w.rb_rows;
+}
+
+template <typename Tag, int KV, int D, int R, bool SMALL>
+hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
+  using C = AttnCfg<Tag, KV, D, R, SMALL>;
+  auto kern = paged_attn_kernel<Tag, KV, D, R, SMALL>;
+  hipError_t e = allow_lds((const void*)kern, C::LDS_BYTES);
+  if (e != hipSuccess) return e;
+  const int columns = (a.heads_kv >> a.head_shift) * w.nrb;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(columns * w.shares)), dim3(C::NT), C::LDS_BYTES, stream, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.tickets || w.shares == 1) return e;
+  hipLaunchKernelGGL((paged_merge_kernel<Tag, KV, D, R, SMALL>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
+                     stream, a);
+  return hipGetLastError();
+}
+
+template <typename Tag, int KV, int D>
+hipError_t run_dim(const PagedAttnArgs& a, const Plan& w, hipStream_t s) {
+  if (a.shift < 4) return run<Tag, KV, D, 1, true>(a, w, s);
+  if constexpr (KV != FA_KV_SAME && D <= 128) {
+    if (w.r == 4) return run<Tag, KV, D, 4, false>(a, w, s);
+    if (w.r == 2) return run<Tag, KV, D, 2, false>(a, w, s);
+  }
+  return run<Tag, KV, D, 1, false>(a, w, s);
+}
+
+template <typename Tag, int KV>
+hipError_t run_format(const PagedAttnArgs& a, const Plan& w, int dim, hipStream_t s) {
+  switch (dim) {
+    case 32: return run_dim<Tag, KV, 32>(a, w, s);
+    case 64: return run_dim<Tag, KV, 64>(a, w, s);
+    case 128: return run_dim<Tag, KV, 128>(a, w, s);
+    case 256: return run_dim<Tag, KV, 256>(a, w, s);
+    case 512: return run_dim<Tag, KV, 512>(a, w, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+size_t paged_blocks_workspace_bytes(const fa_paged_blocks_params& p) {
+  const Plan w = plan_of(p);
+  return (size_t)partial_rows(p, w) * (p.head_dim + 2) * sizeof(float);
+}
+
+hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
+  const Plan w = plan_of(p);
+  // The kernel's grid is one row of workgroups.
+  if ((int64_t)(p.heads_kv >> w.head_shift) * w.nrb * w.shares > INT_MAX) return hipErrorInvalidValue;
+  PagedAttnArgs a{};
+  a.q = p.q;
+  a.out = p.out;
+  a.k = p.k_cache;
+  a.v = p.v_cache;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = p.q_stride[i];
+    a.out_stride[i] = p.out_stride[i];
+    a.k_stride[i] = p.k_stride[i];
+    a.v_stride[i] = p.v_stride[i];
+    a.index_stride[i] = p.block_index_stride[i];
+  }
+  a.table = p.block_table;
+  a.lens = p.context_lens;
+  a.lens_stride = p.context_lens_stride;
+  a.ks = p.k_scale;
+  a.vs = p.v_scale;
+  for (int i = 0; i < 2; ++i) {
+    a.table_stride[i] = p.block_table_stride[i];
+    a.ks_stride[i] = p.k_scale_stride[i];
+    a.vs_stride[i] = p.v_scale_stride[i];
+  }
+  a.index = p.block_index;
+  a.n_index = p.n_index;
+  a.num_blocks = p.num_blocks;
+  a.max_blocks = p.max_blocks;
+  a.shift = log2_floor(p.block_size);
+  a.batch = p.batch;
+  a.heads_q = p.heads_q;
+  a.heads_kv = p.heads_kv;
+  a.seqlen_q = p.seqlen_q;
+  a.bf16 = p.dtype == FA_DTYPE_BF16;
+  a.scale_log2 = p.softmax_scale * kLog2e;
+  a.causal = p.causal;
+  a.shares = w.shares;
+  a.head_shift = w.head_shift;
+  a.ws_o = reinterpret_cast<float*>(p.workspace);
+  a.ws_ml = a.ws_o + partial_rows(p, w) * p.head_dim;
+  a.tickets = p.tickets;
+  // (8-bit caches: the kernels' products are fp16 for either query type.)
+  switch (p.kv_format) {
+    case FA_KV_E4M3: return run_format<f16_t, FA_KV_E4M3>(a, w, p.head_dim, s);
+    case FA_KV_INT8: return run_format<f16_t, FA_KV_INT8>(a, w, p.head_dim, s);
+    case FA_KV_SAME:
+      return a.bf16 ? run_format<bf16_t, FA_KV_SAME>(a, w, p.head_dim, s) : run_format<f16_t, FA_KV_SAME>(a, w, p.head_dim, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace fa

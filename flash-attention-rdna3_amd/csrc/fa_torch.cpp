@@ -23,6 +23,8 @@
 //   paged_allocate(block_table, context_lens, ...) -> (slots, cu_seqlens, next_head)
 //   paged_append(key, value, k_cache, v_cache, slots, ...)   in place
 //   paged_select(query, key_bounds, block_table, ...) -> index
+//   decode_paged_blocks(q, k_cache, v_cache, block_table, context_lens, k_scale?, v_scale?, block_index?, ...) -> out
+//             paged decode over 8-bit caches with block scales, and over listed blocks
 //   set_ds_scratch_limit(bytes) / ds_scratch_limit() -> bytes
 // Argument contracts are checked by the Python layer with the reference's
 // messages before any of these is called; the C ABI re-checks what could
@@ -755,6 +757,76 @@ Tensor paged_select_op(const Tensor& query, const Tensor& key_bounds, const Tens
   return index;
 }
 
+Tensor decode_paged_blocks_op(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                              const Tensor& block_table, const Tensor& context_lens, const OptTensor& k_scale,
+                              const OptTensor& v_scale, const OptTensor& block_index, bool causal, double scale,
+                              int64_t shares, const OptTensor& tickets) {
+  check_16bit(query, "query");
+  const int format = kv_format_of(k_cache, query);
+  TORCH_CHECK(query.dim() == 4, "fa_mi355x: query must be (batch, heads, rows, head_dim)");
+  for (const Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->device() == query.device() && t->dim() == 4 && t->sizes() == k_cache.sizes() &&
+                    t->scalar_type() == k_cache.scalar_type() && t->size(3) == query.size(3),
+                "fa_mi355x: caches must be (blocks, block_size, heads_kv, head_dim) of one shape and dtype, on the "
+                "query's device");
+  if (format != FA_KV_SAME) check_scales(k_scale, v_scale, k_cache);
+  TORCH_CHECK(block_table.dim() == 2, "fa_mi355x: block_table must be 2-D");
+  check_int32(block_table, query, {query.size(0), block_table.size(1)}, "block_table");
+  check_int32(context_lens, query, {query.size(0)}, "context_lens");
+  if (block_index.has_value()) {
+    TORCH_CHECK(block_index->dim() == 3, "fa_mi355x: block_index must be 3-D");
+    check_int32(*block_index, query, {query.size(0), k_cache.size(2), block_index->size(2)}, "block_index");
+  }
+  check_tickets(tickets, query);
+  c10::DeviceGuard guard(query.device());
+  const Tensor q = kernel_ready(query), k = kernel_ready(k_cache), v = kernel_ready(v_cache);
+  const Tensor out = at::empty(q.sizes(), q.options());
+  fa_paged_blocks_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.abi_version = FA_ABI_VERSION;
+  p.dtype = dtype_code(q.scalar_type());
+  p.q = q.data_ptr();
+  p.k_cache = k.data_ptr();
+  p.v_cache = v.data_ptr();
+  p.out = out.data_ptr();
+  p.block_table = block_table.data_ptr<int32_t>();
+  p.context_lens = context_lens.data_ptr<int32_t>();
+  abi_strides(p.q_stride, q, true);
+  abi_strides(p.k_stride, k, true);
+  abi_strides(p.v_stride, v, true);
+  abi_strides(p.out_stride, out, true);
+  abi_strides(p.block_table_stride, block_table);
+  p.context_lens_stride = context_lens.stride(0);
+  if (format != FA_KV_SAME) {
+    p.k_scale = k_scale->data_ptr<float>();
+    p.v_scale = v_scale->data_ptr<float>();
+    abi_strides(p.k_scale_stride, *k_scale);
+    abi_strides(p.v_scale_stride, *v_scale);
+  }
+  if (block_index.has_value()) {
+    p.block_index = block_index->data_ptr<int32_t>();
+    abi_strides(p.block_index_stride, *block_index);
+    p.n_index = to_int32(block_index->size(2), "block_index");
+  }
+  p.batch = to_int32(q.size(0), "batch");
+  p.heads_q = to_int32(q.size(1), "heads");
+  p.heads_kv = to_int32(k.size(2), "heads_kv");
+  p.head_dim = to_int32(q.size(3), "head_dim");
+  p.num_blocks = to_int32(k.size(0), "blocks");
+  p.block_size = to_int32(k.size(1), "block_size");
+  p.max_blocks = to_int32(block_table.size(1), "blocks of a sequence");
+  p.seqlen_q = to_int32(q.size(2), "rows");
+  p.kv_format = format;
+  p.softmax_scale = (float)scale;
+  p.causal = causal ? 1 : 0;
+  p.shares = to_int32(shares, "shares");
+  const Tensor ws = at::empty({(int64_t)fa_paged_blocks_workspace_bytes(&p)}, q.options().dtype(at::kByte));
+  p.workspace = ws.data_ptr();
+  if (tickets.has_value()) p.tickets = reinterpret_cast<uint32_t*>(tickets->data_ptr<int32_t>());
+  check_status(fa_decode_paged_blocks(&p, stream_of(query)), "fa_decode_paged_blocks");
+  return out;
+}
+
 // Inside a torch.func transform.  Decode has no rule for any of them, and a
 // wrapped argument must not reach it: a jvp would come back with a silent zero
 // tangent.  Plain tensors are not the transform's business.
@@ -776,7 +848,8 @@ int64_t set_ds_scratch_limit(int64_t bytes) {
 int64_t ds_scratch_limit() { return g_ds_limit.load(); }
 
 // Operators that stay outside autograd and torch.func.
-constexpr const char* kInferenceOnly[] = {"decode", "decode_paged", "paged_allocate", "paged_append", "paged_select"};
+constexpr const char* kInferenceOnly[] = {"decode",       "decode_paged", "paged_allocate",
+                                            "paged_append", "paged_select", "decode_paged_blocks"};
 
 }  // namespace
 
@@ -798,6 +871,9 @@ TORCH_LIBRARY(fa_mi355x, m) {
         "Tensor(c!)? k_scale, Tensor(d!)? v_scale, Tensor(e!)? key_bounds) -> ()");
   m.def("paged_select(Tensor query, Tensor key_bounds, Tensor block_table, Tensor context_lens, int num_selected, "
         "int block_size, int keep_first, int keep_last) -> Tensor");
+  m.def("decode_paged_blocks(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, "
+        "Tensor? k_scale, Tensor? v_scale, Tensor? block_index, bool causal, float scale, int shares, "
+        "Tensor(a!)? tickets) -> Tensor");
   m.def("set_ds_scratch_limit(int bytes) -> int", &set_ds_scratch_limit);
   m.def("ds_scratch_limit() -> int", &ds_scratch_limit);
 }
@@ -812,6 +888,7 @@ TORCH_LIBRARY_IMPL(fa_mi355x, CUDA, m) {
   m.impl("paged_allocate", &paged_allocate_op);
   m.impl("paged_append", &paged_append_op);
   m.impl("paged_select", &paged_select_op);
+  m.impl("decode_paged_blocks", &decode_paged_blocks_op);
 }
 
 // Decode is inference-only: like a launch on raw pointers, its output and the

@@ -189,6 +189,7 @@ EXPORTS = (
     "fa_fwd", "fa_fwd_ws", "fa_fwd_workspace_bytes", "fa_bwd", "fa_bwd_phase", "fa_bwd_workspace_bytes", "fa_bwd_workspace_min_bytes", "fa_decode_splitk", "fa_decode_splitk_noalloc", "fa_decode_paged",
     "fa_tiny_fwd_f32",
     "fa_kvcache_append",
+    "fa_decode_paged_blocks", "fa_paged_blocks_workspace_bytes",
     "fa_paged_allocate", "fa_paged_append", "fa_paged_select", "fa_select_workspace_bytes",
     "fa_hbm_read_probe_count", "fa_hbm_read_probe_name", "fa_hbm_read_probe",
 )
@@ -235,11 +236,14 @@ def lib():
                              ("fa_decode_splitk", DecodeParams), ("fa_decode_splitk_noalloc", DecodeParams),
                              ("fa_decode_paged", PagedParams),
                              ("fa_tiny_fwd_f32", TinyParams), ("fa_kvcache_append", AppendParams),
+                             ("fa_decode_paged_blocks", PagedBlocksParams),
                              ("fa_paged_allocate", AllocateParams), ("fa_paged_append", PagedAppendParams),
                              ("fa_paged_select", SelectParams)):
             fn = getattr(handle, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(struct), ctypes.c_void_p]
+        handle.fa_paged_blocks_workspace_bytes.restype = ctypes.c_size_t
+        handle.fa_paged_blocks_workspace_bytes.argtypes = [ctypes.c_void_p]
         handle.fa_select_workspace_bytes.restype = ctypes.c_size_t
         handle.fa_select_workspace_bytes.argtypes = [ctypes.c_int] * 3
         handle.fa_bwd_phase.restype = ctypes.c_int

@@ -331,3 +331,31 @@ def validate_select_inputs(query, key_bounds, block_table, context_lens, num_sel
     if keep_first + keep_last > num_selected:
         raise ValueError("keep_first + keep_last must not exceed num_selected")
     _require_platform(device)
+
+
+def validate_paged_blocks_inputs(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, block_index):
+    """Contracts of the paged decode over block scales and a block index, for
+    a 4-D query: the paged shape rules, checked on stand-ins of the query's
+    type, and the rules of scales and index."""
+    if query.dtype not in LOW_PRECISION_DTYPES:
+        raise ValueError("query must be float16 or bfloat16")
+    _require_tensor("k_cache", k_cache)
+    _require_tensor("v_cache", v_cache)
+    eight = k_cache.dtype in EIGHT_BIT_DTYPES
+    if k_cache.dtype != v_cache.dtype or not (eight or k_cache.dtype == query.dtype):
+        raise ValueError("k_cache and v_cache must share a dtype: the query's, float8_e4m3fn or int8")
+    stand_in = lambda t: torch.empty_strided(t.shape, [0] * t.dim(), dtype=query.dtype, device=t.device)  # noqa: E731
+    if query.shape[-1] not in EIGHT_BIT_HEAD_DIMS:
+        raise ValueError("block scales and block_index need head_dim 32, 64, 128, 256 or 512")
+    if k_cache.dim() == 4:
+        _require_block_size(k_cache.shape[1])
+        if eight:
+            for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+                _require_like(name, scale, torch.float32, (k_cache.shape[0], k_cache.shape[2]), query.device)
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale and v_scale apply to float8_e4m3fn and int8 caches only")
+        if block_index is not None:
+            _require_like("block_index", block_index, torch.int32, (query.shape[0], k_cache.shape[2], None), query.device)
+            if block_index.shape[2] <= 0:
+                raise ValueError("block_index must list at least one block")
+    validate_paged_inputs(query.select(2, 0), stand_in(k_cache), stand_in(v_cache), block_table, context_lens)

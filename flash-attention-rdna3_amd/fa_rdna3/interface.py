@@ -29,6 +29,7 @@ from ._validation import (
     validate_attention_options,
     validate_dense_inputs,
     validate_inference_only,
+    validate_paged_blocks_inputs,
     validate_paged_inputs,
     validate_softmax_scale,
     validate_varlen_inputs,
@@ -690,7 +691,7 @@ def flash_attention_varlen(query, key, value, cu_seqlens_q, cu_seqlens_k,
 
 def flash_attention_decode_paged(query, k_cache, v_cache, block_table, context_lens,
                                  softmax_scale=None, *, max_context_len=None, num_splits=None, k_scale=None,
-                                 v_scale=None):
+                                 v_scale=None, block_index=None):
     """Decode attention over a paged (block-table) KV cache, vLLM style.
 
     Args:
@@ -707,8 +708,22 @@ def flash_attention_decode_paged(query, k_cache, v_cache, block_table, context_l
 
     ``k_cache`` / ``v_cache`` may be ``torch.float8_e4m3fn`` caches holding
     K / k_scale and V / v_scale (head_dim 32, 64, 128, 256 or 512; an
-    MI355X-build extension, see :func:`flash_attention_decode`).
+    MI355X-build extension, see :func:`flash_attention_decode`), or 8-bit
+    caches (``torch.float8_e4m3fn`` or ``torch.int8``) with float32 tensors
+    ``k_scale``, ``v_scale`` ``(num_blocks, kv_heads)`` of what the codes of
+    each block and head are multiplied by (:func:`paged_kvcache_append`).
+
+    ``block_index`` (int32 ``(batch, kv_heads, n)``) lists the logical blocks
+    that the query heads of each KV head attend, in place of all blocks of the
+    sequence (:func:`paged_kvcache_select`); entries outside
+    ``[0, ceil(context_len / block_size))`` are no block, one that is listed
+    twice counts twice.  Keys keep the positions of their blocks.
     """
+    if _wants_blocks(k_cache, k_scale, v_scale, block_index):
+        _require_tensor_dims(query, 3)
+        out = _paged_blocks(query.unsqueeze(2), k_cache, v_cache, block_table, context_lens, softmax_scale,
+                            max_context_len, num_splits, False, k_scale, v_scale, block_index)
+        return out.squeeze(2)
     fp8 = _validate_paged(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale)
     validate_inference_only(query, k_cache, v_cache)
     validate_softmax_scale(softmax_scale)
@@ -742,6 +757,40 @@ def _check_fp8_pair(value, k_scale, v_scale):
         if sc is not None and (isinstance(sc, bool) or not isinstance(sc, (int, float))
                                or not math.isfinite(float(sc)) or float(sc) <= 0.0):
             raise ValueError(f"{name} must be a positive finite number or None")
+
+
+def _wants_blocks(k_cache, k_scale, v_scale, block_index):
+    """Whether a paged call is one over block scales or listed blocks."""
+    return (block_index is not None or isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor)
+            or (isinstance(k_cache, torch.Tensor) and k_cache.dtype == torch.int8))
+
+
+def _require_tensor_dims(query, dims):
+    if not isinstance(query, torch.Tensor) or query.dim() != dims:
+        raise ValueError("paged query must be (batch, heads, dim) and caches must be (blocks, block, heads, dim)")
+
+
+def _paged_blocks(query, k_cache, v_cache, block_table, context_lens, softmax_scale, max_context_len, num_splits,
+                  causal, k_scale, v_scale, block_index):
+    """Checks and launch of a (batch, q_heads, Sq, head_dim) query over block
+    scales or listed blocks."""
+    if isinstance(k_cache, torch.Tensor) and k_cache.dtype == torch.float8_e4m3fn and k_cache.dim() == 4:
+        if not isinstance(k_scale, torch.Tensor) and not isinstance(v_scale, torch.Tensor):
+            # Listed blocks of a cache with one scale for all of them.
+            _check_fp8_pair(v_cache, k_scale, v_scale)
+            shape = (k_cache.shape[0], k_cache.shape[2])
+            k_scale, v_scale = (torch.full((1, 1), 1.0 if s is None else float(s), device=k_cache.device).expand(shape)
+                                for s in (k_scale, v_scale))
+    validate_paged_blocks_inputs(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, block_index)
+    validate_inference_only(query, k_cache, v_cache)
+    validate_softmax_scale(softmax_scale)
+    _paged_options(max_context_len, num_splits)
+    batch, q_heads, seqlen_q, head_dim = query.shape
+    softmax_scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
+    shares = 0 if num_splits is None else min(4096, int(num_splits) * batch)
+    return _native.ops().decode_paged_blocks(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale,
+                                             block_index, causal, softmax_scale, shares,
+                                             _native.decode_tickets(query, batch, q_heads, seqlen_q))
 
 
 def _paged_options(max_context_len, num_splits):
@@ -784,7 +833,7 @@ def _paged_launch(query, k_cache, v_cache, block_table, context_lens, softmax_sc
 
 def flash_attention_decode_paged_multi(query, k_cache, v_cache, block_table, context_lens, softmax_scale=None,
                                        *, causal=True, max_context_len=None, num_splits=None, k_scale=None,
-                                       v_scale=None):
+                                       v_scale=None, block_index=None):
     """Paged decode of several query rows per sequence (speculative or chunked
     decode over a vLLM-style cache; no counterpart in the reference, whose
     paged decode takes one row, interface.py:643-728).
@@ -793,9 +842,14 @@ def flash_attention_decode_paged_multi(query, k_cache, v_cache, block_table, con
     :func:`flash_attention_decode_paged`, with ``context_lens`` counting the
     query rows' own keys (already written to their pages).  ``causal`` aligns
     bottom-right per sequence: row ``i`` sees keys ``j <= context_len - Sq + i``.
+    Scales and ``block_index`` (one list for all rows) are those of
+    :func:`flash_attention_decode_paged` too.
     Returns ``(batch, q_heads, Sq, head_dim)``.  Inference-only.
     """
     _require_4d_query(query)
+    if _wants_blocks(k_cache, k_scale, v_scale, block_index):
+        return _paged_blocks(query, k_cache, v_cache, block_table, context_lens, softmax_scale, max_context_len,
+                             num_splits, bool(causal), k_scale, v_scale, block_index)
     fp8 = _validate_paged(query.select(2, 0), k_cache, v_cache, block_table, context_lens, k_scale, v_scale)
     validate_inference_only(query, k_cache, v_cache)
     validate_softmax_scale(softmax_scale)

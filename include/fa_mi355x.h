@@ -347,7 +347,8 @@ typedef struct fa_paged_blocks_params {
   int32_t kv_format; /* fa_kv_format */
   float softmax_scale;
   int32_t causal;
-  int32_t shares;    /* workgroups that share the keys of one (KV head, row block); 1..4096 */
+  int32_t shares;    /* workgroups that share the keys of one (KV head, row block), up to 4096; 0: the
+                        library's choice */
   int32_t reserved0;
   void* workspace;   /* fa_paged_blocks_workspace_bytes(params) bytes, 16-byte aligned */
   uint32_t* tickets; /* NULL: the shares are merged by a second launch; else
@@ -554,6 +555,10 @@ int fa_decode_splitk(const fa_decode_params* params, void* stream);
 #define FA_NOALLOC_TICKETS 65536
 int fa_decode_splitk_noalloc(const fa_decode_params* params, void* stream);
 int fa_decode_paged(const fa_paged_params* params, void* stream);
+/* Scratch of fa_decode_paged_blocks (it depends on shares, the shape and, with
+ * shares 0, the current device's compute units). */
+size_t fa_paged_blocks_workspace_bytes(const fa_paged_blocks_params* params);
+int fa_decode_paged_blocks(const fa_paged_blocks_params* params, void* stream);
 int fa_paged_allocate(const fa_allocate_params* params, void* stream);
 int fa_paged_append(const fa_paged_append_params* params, void* stream);
 size_t fa_select_workspace_bytes(int batch, int heads_kv, int max_blocks);

@@ -7,7 +7,14 @@ import numpy as np
 import pytest
 import torch
 
-from fa_rdna3 import _native, paged_kvcache_allocate, paged_kvcache_append, paged_kvcache_select
+from fa_rdna3 import (
+    _native,
+    flash_attention_decode_paged,
+    flash_attention_decode_paged_multi,
+    paged_kvcache_allocate,
+    paged_kvcache_append,
+    paged_kvcache_select,
+)
 from oracle import paged_cache as oracle
 from paged_cases import int32
 
@@ -183,3 +190,88 @@ def test_oracle_block_scales_and_index_reduce_to_the_plain_paged_decode():
                         np.tile(np.arange(4), (2, 2, 1)), causal=True)
     want = attention.paged_attention(q, k, v, table, np.array(lens), causal=True)
     np.testing.assert_allclose(got, want, atol=1e-5)
+
+
+# ---------------------------------------------------------------------------
+# Paged decode over block scales and listed blocks
+# ---------------------------------------------------------------------------
+
+def _decode_args(cache=torch.int8, dim=64, index=True):
+    shape = (9, 16, 2, dim)
+    return dict(query=torch.zeros(2, 8, dim, dtype=torch.float16), k_cache=torch.zeros(shape).to(cache),
+                v_cache=torch.zeros(shape).to(cache), block_table=torch.zeros(2, 4, dtype=torch.int32),
+                context_lens=int32([40, 64]), k_scale=torch.ones(9, 2), v_scale=torch.ones(9, 2),
+                block_index=torch.zeros(2, 2, 3, dtype=torch.int32) if index else None)
+
+
+@pytest.mark.parametrize("cache,scales,index", [
+    (torch.int8, True, False), (torch.int8, True, True), (torch.float8_e4m3fn, True, False),
+    (torch.float8_e4m3fn, False, True), (torch.float16, False, True)])
+@pytest.mark.parametrize("rows", [0, 3])
+def test_complete_decodes_reach_the_platform_check(cache, scales, index, rows):
+    args = _decode_args(cache, index=index)
+    if not scales:
+        args["k_scale"] = args["v_scale"] = None
+    if rows:
+        args["query"] = torch.zeros(2, 8, rows, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="requires|supports"):
+        (flash_attention_decode_paged_multi if rows else flash_attention_decode_paged)(**args)
+
+
+@pytest.mark.parametrize("argument,change,message", [
+    ("query", lambda t: t.float(), "float16 or bfloat16"), ("query", lambda t: t[0], "paged query must be"),
+    ("query", lambda t: t[..., :48], "need head_dim"), ("query", lambda t: t[..., :32], "head_dim"),
+    ("query", lambda t: t[:, :7], "multiple of cache heads"), ("query", lambda t: None, "paged query must be"),
+    ("k_cache", lambda t: t.half(), "share a dtype"), ("k_cache", lambda t: t[0], "caches must be"),
+    ("v_cache", lambda t: t[:5], "same shape"), ("v_cache", lambda t: t.to(torch.float8_e4m3fn), "share a dtype"),
+    ("k_scale", lambda t: 1.0, "k_scale must be a torch.Tensor"), ("v_scale", lambda t: None, "v_scale must be"),
+    ("k_scale", lambda t: t.half(), "k_scale must be"), ("v_scale", lambda t: t[:, :1], "v_scale must be"),
+    ("k_scale", lambda t: t[:4], "k_scale must be"),
+    ("block_index", lambda t: t.long(), "block_index must be"), ("block_index", lambda t: t[0], "block_index must be"),
+    ("block_index", lambda t: t[:, :1], "block_index must be"), ("block_index", lambda t: t[..., :0], "at least one block"),
+    ("block_table", lambda t: t.long(), "block_table must be"), ("context_lens", lambda t: t[:1], "context_lens"),
+])
+def test_refused_decodes(argument, change, message):
+    args = _decode_args()
+    args[argument] = change(args[argument])
+    with pytest.raises((ValueError, TypeError), match=message):
+        flash_attention_decode_paged(**args)
+
+
+def test_refused_decodes_by_cache():
+    args = _decode_args(torch.float16)
+    with pytest.raises(ValueError, match="apply to"):
+        flash_attention_decode_paged(**args)
+    args = _decode_args(torch.float8_e4m3fn) | {"k_scale": 0.5}
+    with pytest.raises(TypeError, match="k_scale"):
+        flash_attention_decode_paged(**args)
+    args = _decode_args(torch.float8_e4m3fn) | {"k_scale": -0.5, "v_scale": None}
+    with pytest.raises(ValueError, match="positive finite"):
+        flash_attention_decode_paged(**args)
+    args = _decode_args(torch.float16, 16) | {"k_scale": None, "v_scale": None}
+    with pytest.raises(ValueError, match="need head_dim"):
+        flash_attention_decode_paged(**args)
+    args = _decode_args()
+    for bad in (0, 33, True):
+        with pytest.raises((ValueError, RuntimeError)):
+            flash_attention_decode_paged(**args, num_splits=bad)
+
+
+def test_paged_blocks_entry_point_checks_before_it_launches():
+    lib = _native.lib()
+    assert lib.fa_decode_paged_blocks(None, None) == 1
+    p = _native.PagedBlocksParams()
+    assert lib.fa_decode_paged_blocks(ctypes.byref(p), None) == 1 and b"abi_version" in lib.fa_last_error_string()
+    p.abi_version, p.kv_format, p.head_dim = _native.ABI_VERSION, 2, 64
+    p.batch, p.heads_q, p.heads_kv, p.seqlen_q = 2, 8, 2, 1
+    p.num_blocks, p.max_blocks, p.block_size, p.shares = 9, 4, 16, 5
+    assert lib.fa_decode_paged_blocks(ctypes.byref(p), None) == 1 and b"rows" in lib.fa_last_error_string()
+    # two partials for each share, KV head and query row of its group: D sums, a maximum and a total
+    assert lib.fa_paged_blocks_workspace_bytes(ctypes.byref(p)) == 2 * 5 * 2 * 4 * (64 + 2) * 4
+    for field, value, status in (("kv_format", 3, 1), ("head_dim", 48, 2), ("block_size", 24, 1), ("shares", 4097, 1),
+                                 ("max_blocks", 2 ** 27, 2), ("heads_kv", 3, 1), ("batch", 70000, 1)):
+        old = getattr(p, field)
+        setattr(p, field, value)
+        assert lib.fa_decode_paged_blocks(ctypes.byref(p), None) == status, field
+        assert lib.fa_paged_blocks_workspace_bytes(ctypes.byref(p)) == 0, field
+        setattr(p, field, old)
