@@ -17,11 +17,11 @@ int log2_floor(int n) {
 int row_blocks(const fa_paged_blocks_params& p) {
   const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
   if (p.kv_format == FA_KV_SAME || p.head_dim > 128 || p.block_size < 16 || rows <= 16) return 1;
-  return rows <= 32 ? 2 : 4;
+  return 2;
 }
 
 struct Plan {
-  int r, head_shift, nrb, rb_rows, shares;
+  int r, nrb, rb_rows, shares;
 };
 
 Plan plan_of(const fa_paged_blocks_params& p) {
@@ -30,11 +30,7 @@ Plan plan_of(const fa_paged_blocks_params& p) {
   const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
   w.nrb = (int)((rows + 16 * w.r - 1) / (16 * w.r));
   w.rb_rows = (int)std::min<int64_t>(rows, 16 * w.r);
-  w.head_shift = 0;
-#ifdef FA_HEAD_SHIFT
-  w.head_shift = std::min(FA_HEAD_SHIFT, log2_floor(p.heads_kv & -p.heads_kv));
-#endif
-  const int64_t columns = (int64_t)(p.heads_kv >> w.head_shift) * w.nrb;
+  const int64_t columns = (int64_t)p.heads_kv * w.nrb;
   w.shares = p.shares > 0 ? p.shares
                           : (int)std::max<int64_t>(1, (device_cu_count() + columns - 1) / columns);
   return w;
@@ -50,11 +46,11 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
   auto kern = paged_attn_kernel<Tag, KV, D, R, SMALL>;
   hipError_t e = allow_lds((const void*)kern, C::LDS_BYTES);
   if (e != hipSuccess) return e;
-  const int columns = (a.heads_kv >> a.head_shift) * w.nrb;
+  const int columns = a.heads_kv * w.nrb;
   hipLaunchKernelGGL(kern, dim3((unsigned)(columns * w.shares)), dim3(C::NT), C::LDS_BYTES, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.tickets || w.shares == 1) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<Tag, KV, D, R, SMALL>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
+  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, 2 * C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
@@ -63,7 +59,6 @@ template <typename Tag, int KV, int D>
 hipError_t run_dim(const PagedAttnArgs& a, const Plan& w, hipStream_t s) {
   if (a.shift < 4) return run<Tag, KV, D, 1, true>(a, w, s);
   if constexpr (KV != FA_KV_SAME && D <= 128) {
-    if (w.r == 4) return run<Tag, KV, D, 4, false>(a, w, s);
     if (w.r == 2) return run<Tag, KV, D, 2, false>(a, w, s);
   }
   return run<Tag, KV, D, 1, false>(a, w, s);
@@ -91,7 +86,7 @@ size_t paged_blocks_workspace_bytes(const fa_paged_blocks_params& p) {
 hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
   const Plan w = plan_of(p);
   // The kernel's grid is one row of workgroups.
-  if ((int64_t)(p.heads_kv >> w.head_shift) * w.nrb * w.shares > INT_MAX) return hipErrorInvalidValue;
+  if ((int64_t)p.heads_kv * w.nrb * w.shares > INT_MAX) return hipErrorInvalidValue;
   PagedAttnArgs a{};
   a.q = p.q;
   a.out = p.out;
@@ -127,10 +122,10 @@ hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.causal = p.causal;
   a.shares = w.shares;
-  a.head_shift = w.head_shift;
   a.ws_o = reinterpret_cast<float*>(p.workspace);
   a.ws_ml = a.ws_o + partial_rows(p, w) * p.head_dim;
-  a.tickets = p.tickets;
+  // (The merge in the same launch addresses partials by 32-bit offsets.)
+  a.tickets = partial_rows(p, w) * p.head_dim * 4 < (int64_t(1) << 31) ? p.tickets : nullptr;
   // (8-bit caches: the kernels' products are fp16 for either query type.)
   switch (p.kv_format) {
     case FA_KV_E4M3: return run_format<f16_t, FA_KV_E4M3>(a, w, p.head_dim, s);

@@ -12,11 +12,13 @@
 //    end of one sequence, whole ones, and the start of another; sequences that
 //    several shares hold are merged from unnormalised partials by the last
 //    workgroup that arrives (or by a second launch).
-//  * Registers.  A wave streams its chunks through NBUF slots: K in the
-//    layout of the matrix instruction's A operand, V as raw 16-byte pieces
-//    that pass through an LDS tile of the wave and come back transposed.
-//    Page ids and scales are scalar loads, so that they do not wait behind the
-//    stream.  A slot is refilled right after its use.
+//  * Stream.  A wave has one chunk in registers (K in the layout of the matrix
+//    instruction's A operand, V as raw 16-byte pieces that pass through an LDS
+//    tile of the wave and come back transposed) and asks for its next one as
+//    soon as each register is read: V after the tile is written, K after
+//    Q K^T.  Page ids and scales are scalar loads a chunk or two ahead, so that
+//    they do not wait behind the stream.  The step is compiled once: unrolled
+//    over two chunks in flight the code outgrew the instruction cache.
 //  * Types.  8-bit codes are fp16 numbers exactly, so over 8-bit caches the
 //    products run in fp16 whatever the query's type: a bfloat16 query row is
 //    scaled by a power of two to a largest value of 2^14 first (its 8 bits fit;
@@ -60,8 +62,7 @@ struct PagedAttnArgs {
   int32_t batch, heads_q, heads_kv, seqlen_q, bf16;
   float scale_log2;
   int32_t causal;
-  int32_t shares;        // workgroups of a (head group, row block)
-  int32_t head_shift;    // log2 of the KV heads of a workgroup
+  int32_t shares;        // workgroups of a (KV head, row block)
   float* ws_o;           // [2 * shares][heads_kv][row blocks][rows of a block][D]
   float* ws_ml;          // the same without D, pairs (m, l)
   uint32_t* tickets;
@@ -70,8 +71,10 @@ struct PagedAttnArgs {
 template <typename Tag, int KV, int D, int R, bool SMALL>
 struct AttnCfg {
   static constexpr bool KV8 = KV != FA_KV_SAME;
-  static constexpr int NW = (R >= 4 || D == 512 || !KV8) ? 4 : 8;  // waves
+  // Waves: two per SIMD where a chunk and the sums leave room for them.
+  static constexpr int NW = D == 512 || (!KV8 && D == 256) ? 4 : 8;
   static constexpr int NT = 64 * NW;
+  static constexpr int RB = 16 * R;                           // rows of a row block
   static constexpr int NSTEP = D / 32;                        // 32-dim steps of Q K^T
   static constexpr int NDB = D / 16;                          // 16-dim blocks of O
   static constexpr bool PAIR = KV8 && NSTEP > 1;              // one 16-byte K load for two steps
@@ -80,16 +83,12 @@ struct AttnCfg {
   static constexpr int EPP = KV8 ? 16 : 8;                    // elements of a 16-byte V piece
   static constexpr int PPR = D / EPP;                         // pieces of a row
   static constexpr int VN = 32 * PPR / 64;                    // V loads per chunk
-  static constexpr int SLOT = 2 * KN * KREGS + 4 * VN;
   // V of a 16-bit chunk at D = 512 loads at its use: no room for it beside K.
   static constexpr bool VLATE = !KV8 && D == 512;
-  static constexpr int BUDGET = KV8 ? 64 : 128;
-  static constexpr int NBUF = SLOT >= BUDGET ? 1 : BUDGET / SLOT > 4 ? 4 : BUDGET / SLOT;
-  static constexpr int TILE_BYTES = 32 * D * 2;
-  static constexpr int STATE = NDB * 4 + 2;                   // floats of a wave's row block per lane
-  static constexpr int MERGE_BYTES = NW / 2 * R * STATE * 256;
-  static constexpr int LOOP_BYTES = NW * TILE_BYTES;
-  static constexpr int LDS_BYTES = (LOOP_BYTES > MERGE_BYTES ? LOOP_BYTES : MERGE_BYTES) + 16;
+  static constexpr int LOOP_BYTES = NW * 32 * D * 2;          // the V tiles
+  static constexpr int OLD = D + 4;                           // row stride of the waves' sums (floats)
+  static constexpr int MERGE_BYTES = NW * RB * (OLD + 2) * 4;
+  static constexpr int LDS_BYTES = (LOOP_BYTES > MERGE_BYTES ? LOOP_BYTES : MERGE_BYTES) + 16;  // + ticket flag
 };
 
 template <typename Tag> __device__ inline f32x4a mma16x16(s16x8 a, s16x8 b, f32x4a c);
@@ -196,49 +195,132 @@ __device__ inline uint16_t to_out(const PagedAttnArgs& a, float x) {
   return a.bf16 ? Elem<bf16_t>::from_f(x) : Elem<f16_t>::from_f(x);
 }
 
-// Merges the partials of one (sequence, head group, row block): those of
+// Four dims of an output row.
+__device__ inline void store_out(const PagedAttnArgs& a, int b, int hk, int row, int d, const f32x4a& o) {
+  const int group = a.heads_q / a.heads_kv, g = row / a.seqlen_q, m = row - g * a.seqlen_q;
+  uint16_t* const op = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + (hk * group + g) * a.out_stride[1] +
+                       m * a.out_stride[2] + d;
+  s16x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (short)to_out(a, o[e]);
+  *reinterpret_cast<s16x4*>(op) = x;
+}
+
+// Partials of shares that one launch merges are written through to where
+// every XCD sees them and read from there (the XCDs' L2s are not coherent
+// with each other): cache policy "agent scope".
+constexpr int kAgent = 16;
+__device__ inline __amdgpu_buffer_rsrc_t rsrc_of(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, 0x7FFFFFFF, 0x00020000);
+}
+
+// Index of a partial's row block: `slot` 2 * share, + 1 for the share's last
+// sequence if it goes on behind the share.
+__device__ inline int64_t partial_row(const PagedAttnArgs& a, int slot, int hk, int rb, int nrb, int rb_rows) {
+  return (((int64_t)slot * a.heads_kv + hk) * nrb + rb) * rb_rows;
+}
+
+// Merges the partials of one (sequence, KV head, row block): those of the
 // workgroups j0 .. j1, the first of them in its second slot.
 template <int D, int NT, bool AGENT>
-__device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hg, int rb, int nrb, int rb_rows, int j0, int j1,
+__device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hk, int rb, int nrb, int rb_rows, int j0, int j1,
                                       int tid) {
-  const int hpw = 1 << a.head_shift, group = a.heads_q / a.heads_kv, rows = group * a.seqlen_q;
+  const int rows = a.heads_q / a.heads_kv * a.seqlen_q;
   const int here = min(rb_rows, rows - rb * rb_rows);
-  auto ld = [](const float* p) {
-    if constexpr (AGENT) return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    else return *p;
-  };
-  for (int i = tid; i < hpw * here * D; i += NT) {
-    const int d = i % D, r = (i / D) % here, hk = hg * hpw + i / (D * here);
-    float M = kFloor, L = 0.f, o = 0.f;
-    for (int j = j0; j <= j1; j += 8) {
-      float m[8], l[8], x[8];
+  const __amdgpu_buffer_rsrc_t ro = rsrc_of(a.ws_o), rm = rsrc_of(a.ws_ml);
+  typedef float f32x2a __attribute__((ext_vector_type(2)));
+  for (int i = tid; i < here * (D / 4); i += NT) {
+    const int d = i % (D / 4) * 4, r = i / (D / 4);
+    float M = kFloor, L = 0.f;
+    f32x4a o = {0.f, 0.f, 0.f, 0.f};
+    for (int j = j0; j <= j1; j += 4) {
+      f32x2a ml[4];
+      f32x4a x[4];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < 4; ++u) {
         const int jj = min(j + u, j1);
-        const int64_t row = (((int64_t)(2 * jj + (jj == j0 ? 1 : 0)) * a.heads_kv + hk) * nrb + rb) * rb_rows + r;
-        m[u] = ld(a.ws_ml + 2 * row);
-        l[u] = j + u <= j1 ? ld(a.ws_ml + 2 * row + 1) : 0.f;
-        x[u] = ld(a.ws_o + row * D + d);
+        const int64_t row = partial_row(a, 2 * jj + (jj == j0 ? 1 : 0), hk, rb, nrb, rb_rows) + r;
+        if constexpr (AGENT) {
+          // (bit_cast the whole result: subscripting the builtin's vector
+          // directly compiles to one dword load splatted to all four.)
+          ml[u] = __builtin_bit_cast(f32x2a, __builtin_amdgcn_raw_buffer_load_b64(rm, (int)(row * 8), 0, kAgent));
+          x[u] = __builtin_bit_cast(f32x4a, __builtin_amdgcn_raw_buffer_load_b128(ro, (int)((row * D + d) * 4), 0, kAgent));
+        } else {
+          ml[u] = *reinterpret_cast<const f32x2a*>(a.ws_ml + 2 * row);
+          x[u] = *reinterpret_cast<const f32x4a*>(a.ws_o + row * D + d);
+        }
       }
-      float top = M;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) top = fmaxf(top, m[u]);
-      const float s = __builtin_amdgcn_exp2f(M - top);
-      L *= s;
-      o *= s;
-      M = top;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float w = j + u <= j1 ? __builtin_amdgcn_exp2f(m[u] - top) : 0.f;
-        L += w * l[u];
-        if (j + u <= j1) o += w * x[u];
+      for (int u = 0; u < 4; ++u) {
+        if (j + u > j1) break;
+        const float top = fmaxf(M, ml[u][0]);
+        const float s = __builtin_amdgcn_exp2f(M - top), w = __builtin_amdgcn_exp2f(ml[u][0] - top);
+        L = L * s + ml[u][1] * w;
+        o = o * s + x[u] * w;
+        M = top;
       }
     }
-    const int row = rb * rb_rows + r, g = row / a.seqlen_q, q = row - g * a.seqlen_q;
-    uint16_t* const op = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] + (hk * group + g) * a.out_stride[1] +
-                         q * a.out_stride[2];
-    op[d] = to_out(a, L == 0.f ? 0.f : o / L);
+    store_out(a, b, hk, rb * rb_rows + r, d, o * (L == 0.f ? 0.f : 1.f / L));
   }
+}
+
+// What the shares' kernels have in common: which share this is, and its place
+// in the line of chunks.
+struct SharePlace {
+  int hk, rb, share, nrb, rb_rows;
+  // KV heads fastest: neighbours in dispatch order read the same pages (with
+  // the heads of a key range on one XCD instead: 53 us against 50, 4 x 16384 e4m3).
+  __device__ SharePlace(const PagedAttnArgs& a, int rows_of_block) {
+    const int rows = a.heads_q / a.heads_kv * a.seqlen_q;
+    nrb = (rows + rows_of_block - 1) / rows_of_block;
+    rb_rows = min(rows_of_block, rows);
+    hk = blockIdx.x % a.heads_kv;
+    rb = blockIdx.x / a.heads_kv % nrb;
+    share = blockIdx.x / (a.heads_kv * nrb);
+  }
+};
+
+// After a share wrote its partial of sequence b (chunks [begin, begin + all)
+// of the line): the last of the sequence's shares to arrive merges them.
+// Every store is acknowledged (vmcnt 0) before the workgroup's ticket; no
+// workgroup waits for another.
+template <int D, int NT>
+__device__ inline void arrive(const PagedAttnArgs& a, const SharePlace& w, const Shares& cut, int b, int begin, int all,
+                              int* flag, int tid) {
+  wait_vm_all();
+  __syncthreads();
+  const int j0 = cut.owner(begin), j1 = cut.owner(begin + all - 1);
+  if (tid == 0) {
+    uint32_t* const t = a.tickets + ((int64_t)b * a.heads_kv + w.hk) * w.nrb + w.rb;
+    const bool last = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(j1 - j0);
+    if (last) __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  if (*flag) merge_partials<D, NT, true>(a, b, w.hk, w.rb, w.nrb, w.rb_rows, j0, j1, tid);
+}
+
+// A query row of bfloat16 in a lane's s16x8 pieces -> fp16, scaled by a power
+// of two to a largest value in [2^14, 2^15).  Returns the factor that takes
+// the logits back.  (A row with an infinity or NaN has no finite result.)
+template <int N>
+__device__ inline float bf16_row_to_f16(s16x8 (&q)[N], float top) {
+  const int ex = max((int)(__float_as_uint(top) >> 23), 15);
+  const float down = __uint_as_float((uint32_t)max(268 - ex, 1) << 23);  // 2^(14 - (ex - 127))
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[s][e] = (short)Elem<f16_t>::from_f(Elem<bf16_t>::to_f((uint16_t)q[s][e]) * down);
+  return __uint_as_float((uint32_t)(ex - 14) << 23);
+}
+template <int N>
+__device__ inline float bf16_row_top(const s16x8 (&q)[N]) {
+  float top = 0.f;
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Elem<bf16_t>::to_f((uint16_t)q[s][e])));
+  return top;
 }
 
 template <typename Tag, int KV, int D, int R, bool SMALL>
@@ -251,26 +333,19 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, l16 = lane & 15;
-  constexpr int RB = 16 * R;
   const int group = a.heads_q / a.heads_kv, rows = group * a.seqlen_q;
-  const int nrb = (rows + RB - 1) / RB;
-  const int rb_rows = min(RB, rows);
-  const int hpw = 1 << a.head_shift, nhg = a.heads_kv >> a.head_shift;
-  const int streams = C::NW >> a.head_shift;
-  // KV heads fastest: neighbours in dispatch order read the same pages.
-  const int hg = blockIdx.x % nhg, rb = blockIdx.x / nhg % nrb, share = blockIdx.x / (nhg * nrb);
-  const int hw = wave & (hpw - 1), stream = wave >> a.head_shift;
-  const int hk = hg * hpw + hw;
-  const PagedWork work{a, rb_rows, rb};
-  const Shares cut = work.shares(lane, 2 * streams);
-  if (share >= cut.count) return;
-  const int begin = cut.begin(share), end = cut.begin(share + 1);
+  const SharePlace w(a, C::RB);
+  const int hk = w.hk;
+  const PagedWork work{a, w.rb_rows, w.rb};
+  const Shares cut = work.shares(lane, 2 * C::NW);
+  if (w.share >= cut.count) return;
+  const int begin = cut.begin(w.share), end = cut.begin(w.share + 1);
   int b, b_begin;
   work.find(begin, lane, b, b_begin);
 
   const KE* const kbase = reinterpret_cast<const KE*>(a.k) + hk * a.k_stride[2];
   const KE* const vbase = reinterpret_cast<const KE*>(a.v) + hk * a.v_stride[2];
-  uint16_t* const tile = reinterpret_cast<uint16_t*>(smem) + wave * (C::TILE_BYTES / 2);
+  uint16_t* const tile = reinterpret_cast<uint16_t*>(smem) + wave * (32 * D);
   const int mask = (1 << a.shift) - 1;
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   typedef const __attribute__((address_space(4))) float const_f32;
@@ -280,16 +355,112 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
     const int c0 = at - b_begin, cnt = min(end, b_begin + all) - at;
     const int blocks = (len + mask) >> a.shift;           // logical blocks of the sequence
     const int listed = a.index ? a.n_index : blocks;
-    const_i32* const index = (const_i32*)(a.index ? a.index + b * a.index_stride[0] + hk * a.index_stride[1] : nullptr);
-    const_i32* const table = (const_i32*)(a.table + b * a.table_stride[0]);
+    const int32_t* const index = a.index ? a.index + b * a.index_stride[0] + hk * a.index_stride[1] : nullptr;
+    const int32_t* const table = a.table + b * a.table_stride[0];
 
-    // --- Q ---------------------------------------------------------------
+    // --- what a chunk's keys are ------------------------------------------
+    // Two steps ahead of its use a chunk is known by its logical blocks, one
+    // step by its pages.  Pages of 16 keys or more: one each for keys 0 .. 15
+    // and 16 .. 31, scalar loads.  Smaller pages: lane l describes key l % 32.
+    constexpr int NH = SMALL ? 1 : 2;
+    struct Ahead {
+      int logical[NH], page[NH];
+    };
+    struct Meta {
+      uint32_t there;      // bit k: key k of the chunk is one of the sequence's
+      int key0[NH];        // position of the half's first key, or of the lane's
+      float ks[NH], vs[NH];
+      int64_t koff[NH], voff[NH];
+    };
+    auto first_key = [&](int c, int h) { return 32 * c + (SMALL ? lane & 31 : 16 * h); };
+    // The logical block of the listed block that holds key n of the list.
+    auto logical_of = [&](int n) {
+      const int at_list = n >> a.shift;
+      if (!index) return at_list;
+      const int64_t i = (int64_t)min(at_list, listed - 1) * a.index_stride[2];
+      int l;
+      if constexpr (SMALL) l = index[i];
+      else l = ((const_i32*)index)[i];
+      return at_list < listed ? l : -1;
+    };
+    auto page_of = [&](int logical) {
+      const int64_t i = (int64_t)min(max(logical, 0), a.max_blocks - 1) * a.table_stride[1];
+      if constexpr (SMALL) return table[i];
+      else return ((const_i32*)table)[i];
+    };
+    auto describe = [&](int c, const Ahead& x) -> Meta {
+      Meta m;
+      m.there = 0;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const int inside = first_key(c, h) & mask;
+        const bool ok = x.logical[h] >= 0 && x.logical[h] < blocks && x.page[h] >= 0 && x.page[h] < a.num_blocks;
+        const int page = ok ? x.page[h] : 0;
+        m.key0[h] = ok ? (x.logical[h] << a.shift) + inside : 0;
+        m.koff[h] = page * a.k_stride[0] + inside * a.k_stride[1];
+        m.voff[h] = page * a.v_stride[0] + inside * a.v_stride[1];
+        m.ks[h] = m.vs[h] = 1.f;
+        const int here = ok ? len - m.key0[h] : 0;  // keys from this one on
+        if constexpr (SMALL) {
+          if constexpr (C::KV8) {
+            if (a.ks) m.ks[h] = a.ks[page * a.ks_stride[0] + hk * a.ks_stride[1]];
+            if (a.vs) m.vs[h] = a.vs[page * a.vs_stride[0] + hk * a.vs_stride[1]];
+          }
+          m.there = (uint32_t)__builtin_amdgcn_ballot_w64(here > 0);
+        } else {
+          if constexpr (C::KV8) {
+            if (a.ks) m.ks[h] = ((const_f32*)a.ks)[page * a.ks_stride[0] + hk * a.ks_stride[1]];
+            if (a.vs) m.vs[h] = ((const_f32*)a.vs)[page * a.vs_stride[0] + hk * a.vs_stride[1]];
+          }
+          m.there |= (here > 0 ? 0xFFFFu >> (16 - min(here, 16)) : 0u) << (16 * h);
+        }
+        m.vs[h] = here > 0 ? m.vs[h] : 0.f;
+      }
+      return m;
+    };
+    auto far = [&](int64_t x, int from) {  // x of another lane
+      const uint32_t lo = __shfl((uint32_t)x, from, 64), hi = __shfl((uint32_t)(x >> 32), from, 64);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    };
+    KRaw kd[2][C::KN];
+    u32x4 vd[C::VN];
+    auto load_k = [&](const Meta& m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int64_t off;
+        if constexpr (SMALL) off = far(m.koff[0], 16 * h + l16);
+        else off = m.koff[h] + l16 * a.k_stride[1];
+#pragma unroll
+        for (int s = 0; s < C::KN; ++s)
+          kd[h][s] = *reinterpret_cast<const KRaw*>(kbase + off + (C::PAIR ? 64 * s + 16 * g4 : 32 * s + 8 * g4));
+      }
+    };
+    auto load_v = [&](const Meta& m) {
+#pragma unroll
+      for (int i = 0; i < C::VN; ++i) {
+        const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
+        int64_t off;
+        if constexpr (SMALL) off = far(m.voff[0], row);
+        else off = (row < 16 ? m.voff[0] : m.voff[1]) + (row & 15) * a.v_stride[1];
+        vd[i] = *reinterpret_cast<const u32x4*>(vbase + off + col);
+      }
+    };
+    const int mine = cnt > wave ? (cnt - wave + C::NW - 1) / C::NW : 0;
+    auto chunk = [&](int k) { return c0 + wave + C::NW * min(k, max(mine - 1, 0)); };
+    Ahead next, later;  // of the chunks k + 1 and k + 2
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      next.logical[h] = logical_of(first_key(chunk(0), h));
+      later.logical[h] = logical_of(first_key(chunk(1), h));
+    }
+
+    // --- Q -----------------------------------------------------------------
     s16x8 q[R][C::NSTEP];
     float qscale[R];
     int klim[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = rb * RB + 16 * r + l16;
+      const int row = w.rb * C::RB + 16 * r + l16;
       const bool valid = row < rows;
       const int g = valid ? row / a.seqlen_q : 0, m = valid ? row - g * a.seqlen_q : 0;
       klim[r] = a.causal ? len - a.seqlen_q + m : INT_MAX;
@@ -301,152 +472,30 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         const int d = C::PAIR ? 64 * (s / 2) + 16 * g4 + 8 * (s % 2) : 32 * s + 8 * g4;
         q[r][s] = valid ? *reinterpret_cast<const s16x8*>(src + d) : zero_op<f16_t>();
       }
+    }
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      next.page[h] = page_of(next.logical[h]);
+      later.page[h] = page_of(later.logical[h]);
+    }
+    Meta now = describe(chunk(0), next);
+    load_v(now);
+    load_k(now);
+    next = later;
+#pragma unroll
+    for (int h = 0; h < NH; ++h) later.logical[h] = logical_of(first_key(chunk(2), h));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       qscale[r] = a.scale_log2;
       if (C::KV8 && a.bf16) {
-        float top = 0.f;
-#pragma unroll
-        for (int s = 0; s < C::NSTEP; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = fabsf(Elem<bf16_t>::to_f((uint16_t)q[r][s][e]));
-            top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
-          }
+        float top = bf16_row_top(q[r]);
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const int ex = max((int)(__float_as_uint(top) >> 23), 15);
-        const float down = __uint_as_float((uint32_t)(268 - ex) << 23);  // 2^(14 - (ex - 127))
-        qscale[r] *= __uint_as_float((uint32_t)(ex - 14) << 23);
-#pragma unroll
-        for (int s = 0; s < C::NSTEP; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            q[r][s][e] = (short)Elem<f16_t>::from_f(Elem<bf16_t>::to_f((uint16_t)q[r][s][e]) * down);
+        qscale[r] *= bf16_row_to_f16(q[r], top);
       }
     }
 
-    // --- what a chunk's keys are ------------------------------------------
-    // Keys 16h .. 16h + 15 of a chunk (pages of 16 keys or more): one page.
-    struct Half {
-      int page, inside, key0, count;
-      float ks, vs;
-    };
-    auto half_of = [&](int n) -> Half {
-      Half h;
-      const int at_list = n >> a.shift;
-      bool ok = at_list < listed;
-      int logical = at_list;
-      if (a.index) {
-        logical = index[(int64_t)min(at_list, listed - 1) * a.index_stride[2]];
-        ok = ok && logical >= 0;
-      }
-      ok = ok && logical < blocks;
-      const int page = table[(int64_t)min(max(logical, 0), a.max_blocks - 1) * a.table_stride[1]];
-      ok = ok && page >= 0 && page < a.num_blocks;
-      h.page = ok ? page : 0;
-      h.inside = n & mask;
-      h.key0 = ok ? (logical << a.shift) + h.inside : 0;
-      h.count = ok ? min(max(len - h.key0, 0), 16) : 0;
-      h.ks = h.vs = 1.f;
-      if constexpr (C::KV8) {
-        if (a.ks) h.ks = ((const_f32*)a.ks)[h.page * a.ks_stride[0] + hk * a.ks_stride[1]];
-        if (a.vs) h.vs = ((const_f32*)a.vs)[h.page * a.vs_stride[0] + hk * a.vs_stride[1]];
-      }
-      h.vs = h.count ? h.vs : 0.f;
-      return h;
-    };
-    // Pages of fewer keys: lane l describes key l % 32.
-    struct Key {
-      int64_t k, v;
-      int pos, ok;
-      float ks, vs;
-    };
-    auto key_of = [&](int n) -> Key {
-      Key e;
-      const int at_list = n >> a.shift;
-      bool ok = at_list < listed;
-      int logical = at_list;
-      if (a.index) {
-        logical = a.index[b * a.index_stride[0] + hk * a.index_stride[1] + (int64_t)min(at_list, listed - 1) * a.index_stride[2]];
-        ok = ok && logical >= 0;
-      }
-      ok = ok && logical < blocks;
-      int page = a.table[b * a.table_stride[0] + (int64_t)min(max(logical, 0), a.max_blocks - 1) * a.table_stride[1]];
-      ok = ok && page >= 0 && page < a.num_blocks;
-      page = ok ? page : 0;
-      e.pos = ok ? (logical << a.shift) + (n & mask) : 0;
-      e.ok = ok && e.pos < len;
-      e.k = page * a.k_stride[0] + (n & mask) * a.k_stride[1];
-      e.v = page * a.v_stride[0] + (n & mask) * a.v_stride[1];
-      e.ks = e.vs = 1.f;
-      if constexpr (C::KV8) {
-        if (a.ks) e.ks = a.ks[page * a.ks_stride[0] + hk * a.ks_stride[1]];
-        if (a.vs) e.vs = a.vs[page * a.vs_stride[0] + hk * a.vs_stride[1]];
-      }
-      e.vs = e.ok ? e.vs : 0.f;
-      return e;
-    };
-    struct Meta {
-      uint32_t there;         // bit k: key k of the chunk is one of the sequence's
-      int key0[2];
-      float ks[2], vs[2];     // SMALL: of the lane's key, in [0]
-      int64_t voff[SMALL ? 1 : 2];
-    };
-    KRaw kr[C::NBUF][2][C::KN];
-    u32x4 vr[C::NBUF][C::VN];
-    Meta meta[C::NBUF];
-
-    auto load_v = [&](const Meta& m, u32x4 (&vd)[C::VN]) {
-#pragma unroll
-      for (int i = 0; i < C::VN; ++i) {
-        const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
-        int64_t off;
-        if constexpr (SMALL) {
-          const uint32_t lo = __shfl((uint32_t)m.voff[0], row, 64), hi = __shfl((uint32_t)(m.voff[0] >> 32), row, 64);
-          off = (int64_t)(((uint64_t)hi << 32) | lo);
-        } else {
-          off = (row < 16 ? m.voff[0] : m.voff[1]) + (row & 15) * a.v_stride[1];
-        }
-        vd[i] = *reinterpret_cast<const u32x4*>(vbase + off + col);
-      }
-    };
-    auto issue = [&](int c, KRaw (&kd)[2][C::KN], u32x4 (&vd)[C::VN], Meta& m) {
-      int64_t koff[2];
-      if constexpr (SMALL) {
-        const Key e = key_of(32 * c + (lane & 31));
-        m.there = (uint32_t)__builtin_amdgcn_ballot_w64(e.ok != 0);
-        m.key0[0] = e.pos;
-        m.ks[0] = e.ks;
-        m.vs[0] = e.vs;
-        m.voff[0] = e.v;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t lo = __shfl((uint32_t)e.k, 16 * h + l16, 64), hi = __shfl((uint32_t)(e.k >> 32), 16 * h + l16, 64);
-          koff[h] = (int64_t)(((uint64_t)hi << 32) | lo);
-        }
-      } else {
-        m.there = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Half e = half_of(32 * c + 16 * h);
-          m.there |= (e.count ? 0xFFFFu >> (16 - e.count) : 0u) << (16 * h);
-          m.key0[h] = e.key0;
-          m.ks[h] = e.ks;
-          m.vs[h] = e.vs;
-          m.voff[h] = e.page * a.v_stride[0] + e.inside * a.v_stride[1];
-          koff[h] = e.page * a.k_stride[0] + (e.inside + l16) * a.k_stride[1];
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int s = 0; s < C::KN; ++s) {
-          const int d = C::PAIR ? 64 * s + 16 * g4 : 32 * s + 8 * g4;
-          kd[h][s] = *reinterpret_cast<const KRaw*>(kbase + koff[h] + d);
-        }
-      if constexpr (!C::VLATE) load_v(m, vd);
-    };
-
-    // --- state -----------------------------------------------------------
+    // --- the stream ----------------------------------------------------------
     float m_i[R], l_i[R];
     f32x4a acc[R][C::NDB];
 #pragma unroll
@@ -457,48 +506,62 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
       for (int i = 0; i < C::NDB; ++i) acc[r][i] = f32x4a{0.f, 0.f, 0.f, 0.f};
     }
     uint32_t vref = 0x00800000u;  // bits of a power of two
+    // Elements that are not finite: (x & ABS) + UP has the top bit set.
+    constexpr uint32_t ABS = C::KV8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
+    constexpr uint32_t UP = C::KV8 ? 0x01010101u : std::is_same<CT, bf16_t>::value ? 0x00800080u : 0x04000400u;
+    uint32_t odd = 0;  // such a value was left out
+    auto is_mixed = [&](const Meta& m) {
+      bool x = a.causal && a.seqlen_q > 1;
+      if constexpr (!SMALL) x = x && max(m.key0[0], m.key0[NH - 1]) + 15 > len - a.seqlen_q;
+      return x;
+    };
 
-    auto compute = [&](const KRaw (&kd)[2][C::KN], const u32x4 (&vd)[C::VN], const Meta& m) {
+#pragma unroll 1
+    for (int k = 0; k < mine; ++k) {
+      const bool more = k + 1 < mine;
+      const Meta m = now;
       const bool whole = m.there == 0xFFFFFFFFu;
-      // V to the tile; rows that are no keys as zeros (0 * NaN would be NaN).
-      // `part`, see below: 0 all values; 1 finite ones, others 0; 2 a one for
-      // each +inf or NaN; 3 a one for each -inf or NaN.
-      auto piece_of = [&](int i) {
-        const int row = (64 * i + lane) / C::PPR;
-        u32x4 x = vd[i];
-        if (!whole && !((m.there >> row) & 1u)) x = u32x4{0, 0, 0, 0};
-        return x;
-      };
-      auto part_of = [&](s16x8 x, int part) {
-        constexpr uint16_t EXP = std::is_same<CT, bf16_t>::value ? 0x7F80 : 0x7C00;
-        const short one = (short)Elem<CT>::from_f(1.f);
+      // Some rows see keys of the chunk that others do not.
+      const bool mixed = is_mixed(m);
+      if constexpr (C::VLATE) load_v(m);
+      // Rows that are no keys as zeros (0 * NaN would be NaN).
+      if (!whole) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint16_t u = (uint16_t)x[e];
-          const bool odd = (u & EXP) == EXP, nan = (u & 0x7FFF) > EXP;
-          const bool hit = odd && (nan || (u >> 15) == (part == 3));
-          x[e] = part == 1 ? (odd ? (short)0 : x[e]) : hit ? one : (short)0;
-        }
-        return x;
-      };
-      auto fill = [&](int part) {
+        for (int i = 0; i < C::VN; ++i)
+          if (!((m.there >> ((64 * i + lane) / C::PPR)) & 1u)) vd[i] = u32x4{0, 0, 0, 0};
+      }
+      // Values that are not finite must not reach the rows that do not see
+      // their keys either: they are left out here, and added behind the loop.
+      if (KV != FA_KV_INT8 && mixed) {
 #pragma unroll
-        for (int i = 0; i < C::VN; ++i) {
-          const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
-          const u32x4 x = piece_of(i);
-          if constexpr (C::KV8) {
-            s16x8 lo = codes_to_f16<KV>(u32x2{x[0], x[1]}), hi = codes_to_f16<KV>(u32x2{x[2], x[3]});
-            if (part) { lo = part_of(lo, part); hi = part_of(hi, part); }
-            *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = lo;
-            *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col + 8)) = hi;
-          } else {
-            s16x8 y = __builtin_bit_cast(s16x8, x);
-            if (part) y = part_of(y, part);
-            *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = y;
+        for (int i = 0; i < C::VN; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bad = ((vd[i][e] & ABS) + UP) & ~ABS;  // top bit of each such element
+            vd[i][e] &= ~((bad >> (C::KV8 ? 7 : 15)) * (C::KV8 ? 0xFFu : 0xFFFFu));
+            odd |= bad;
           }
+      }
+#pragma unroll
+      for (int i = 0; i < C::VN; ++i) {
+        const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
+        if constexpr (C::KV8) {
+          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = codes_to_f16<KV>(u32x2{vd[i][0], vd[i][1]});
+          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col + 8)) = codes_to_f16<KV>(u32x2{vd[i][2], vd[i][3]});
+        } else {
+          *reinterpret_cast<u32x4*>(tile + swz_off<D>(row, col)) = vd[i];
         }
-      };
-      fill(0);
+      }
+      if (more) {
+        now = describe(chunk(k + 1), next);
+        if constexpr (!C::VLATE) load_v(now);
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          next.logical[h] = later.logical[h];
+          next.page[h] = page_of(later.logical[h]);
+          later.logical[h] = logical_of(first_key(chunk(k + 3), h));
+        }
+      }
       f32x4a s[R][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -506,22 +569,24 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         for (int r = 0; r < R; ++r) s[r][h] = f32x4a{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < C::NSTEP; ++t) {
-          s16x8 k;
+          s16x8 x;
           if constexpr (C::PAIR) {
-            const u32x4 w = __builtin_bit_cast(u32x4, kd[h][t / 2]);
-            k = codes_to_f16<KV>(t % 2 ? u32x2{w[2], w[3]} : u32x2{w[0], w[1]});
+            const u32x4 y = __builtin_bit_cast(u32x4, kd[h][t / 2]);
+            x = codes_to_f16<KV>(t % 2 ? u32x2{y[2], y[3]} : u32x2{y[0], y[1]});
           } else if constexpr (C::KV8) {
-            k = codes_to_f16<KV>(__builtin_bit_cast(u32x2, kd[h][t]));
+            x = codes_to_f16<KV>(__builtin_bit_cast(u32x2, kd[h][t]));
           } else {
-            k = __builtin_bit_cast(s16x8, kd[h][t]);
+            x = __builtin_bit_cast(s16x8, kd[h][t]);
           }
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r][h] = mma16x16<CT>(k, q[r][t], s[r][h]);
+          for (int r = 0; r < R; ++r) s[r][h] = mma16x16<CT>(x, q[r][t], s[r][h]);
         }
       }
+      if (more) load_k(now);
       // Per key: scales (uniform over a half, or the key's own) and position.
-      float ks[2][SMALL ? 4 : 1], w[2][SMALL ? 4 : 1];
-      int pos[2][SMALL ? 4 : 1];
+      constexpr int NI = SMALL ? 4 : 1;
+      float ks[2][NI], wv[2][NI];
+      int pos[2][NI];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if constexpr (SMALL) {
@@ -529,29 +594,28 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
           for (int i = 0; i < 4; ++i) {
             const int key = 16 * h + 4 * g4 + i;
             ks[h][i] = __shfl(m.ks[0], key, 64);
-            w[h][i] = __shfl(m.vs[0], key, 64);
+            wv[h][i] = __shfl(m.vs[0], key, 64);
             pos[h][i] = __shfl(m.key0[0], key, 64);
           }
         } else {
           ks[h][0] = m.ks[h];
-          w[h][0] = m.vs[h];
+          wv[h][0] = m.vs[h];
           pos[h][0] = m.key0[h] + 4 * g4;
         }
       }
       if constexpr (C::KV8) {
-        uint32_t top;
+        uint32_t top = __float_as_uint(m.vs[0]) & 0x7FFFFFFFu;
         if constexpr (SMALL) {
-          top = __float_as_uint(m.vs[0]) & 0x7FFFFFFFu;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
         } else {
-          top = max(__float_as_uint(m.vs[0]) & 0x7FFFFFFFu, __float_as_uint(m.vs[1]) & 0x7FFFFFFFu);
+          top = max(top, __float_as_uint(m.vs[NH - 1]) & 0x7FFFFFFFu);
         }
         top = __builtin_amdgcn_readfirstlane(top);
         if (top > vref) {
-          const uint32_t now = min((top + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u);
-          const float f = __uint_as_float((uint32_t)max((int)(0x3F800000u + vref - now), 0));
-          vref = now;
+          const uint32_t grown = min((top + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u);
+          const float f = __uint_as_float((uint32_t)max((int)(0x3F800000u + vref - grown), 0));
+          vref = grown;
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -561,11 +625,8 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < (SMALL ? 4 : 1); ++i) w[h][i] *= inv;
+          for (int i = 0; i < NI; ++i) wv[h][i] *= inv;
       }
-      // Some rows see keys of the chunk that others do not.
-      bool mixed = a.causal && a.seqlen_q > 1;
-      if constexpr (!SMALL) mixed = mixed && max(m.key0[0], m.key0[1]) + 15 > len - a.seqlen_q;
       const bool masked = SMALL || !whole || mixed;
       s16x8 p[R];
 #pragma unroll
@@ -591,25 +652,22 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         if (__builtin_amdgcn_ballot_w64(top - m_i[r] > 8.f)) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float now = fmaxf(m_i[r], top), f = __builtin_amdgcn_exp2f(m_i[r] - now);
-          m_i[r] = now;
+          const float high = fmaxf(m_i[r], top), f = __builtin_amdgcn_exp2f(m_i[r] - high);
+          m_i[r] = high;
           l_i[r] *= f;
 #pragma unroll
           for (int i = 0; i < C::NDB; ++i) acc[r][i] *= f;
         }
-        uint16_t e[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = __builtin_amdgcn_exp2f(s[r][h][i] - m_i[r]);
             l_i[r] += x;
-            float y = C::KV8 ? x * w[h][SMALL ? i : 0] : x;
+            float y = C::KV8 ? x * wv[h][SMALL ? i : 0] : x;
             if (masked) y = s[r][h][i] == kNegInf ? 0.f : y;  // (0 * a scale that is not finite)
-            e[4 * h + i] = Elem<CT>::from_f(y);
+            p[r][4 * h + i] = (short)Elem<CT>::from_f(y);
           }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[r][i] = (short)e[i];
       }
       const int trow = 4 * g4 + (l16 >> 2);
       typedef __attribute__((address_space(3))) s4a lds_s4;
@@ -619,208 +677,132 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         const s4a hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(t + 16 * D));
         return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       };
-      // A value that is not finite must not reach the rows that do not see
-      // its key as 0 * inf: such a chunk takes the finite values first, then
-      // adds an infinity wherever a row sees one.
-      if constexpr (KV != FA_KV_INT8) {
-        if (mixed) {
-          uint32_t odd = 0;
-#pragma unroll
-          for (int i = 0; i < C::VN; ++i) {
-            const u32x4 x = piece_of(i);
-            constexpr uint32_t ABS = C::KV8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
-            constexpr uint32_t UP = C::KV8 ? 0x01010101u : std::is_same<CT, bf16_t>::value ? 0x00800080u : 0x04000400u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= ((x[e] & ABS) + UP) & ~ABS;
-          }
-          if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-            for (int part = 1; part < 4; ++part) {
-              fill(part);
-#pragma unroll
-              for (int r = 0; r < R; ++r) {
-                s16x8 ones;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  ones[e] = s[r][e / 4][e % 4] == kNegInf ? (short)0 : (short)Elem<CT>::from_f(1.f);
-#pragma unroll
-                for (int i = 0; i < C::NDB; ++i) {
-                  const s16x8 v = v_op(i);
-                  if (part == 1) {
-                    acc[r][i] = mma16x16<CT>(v, p[r], acc[r][i]);
-                  } else {
-                    const f32x4a n = mma16x16<CT>(v, ones, f32x4a{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[r][i][e] += n[e] > 0.f ? (part == 2 ? -kNegInf : kNegInf) : 0.f;
-                  }
-                }
-              }
-            }
-            return;
-          }
-        }
-      }
 #pragma unroll
       for (int i = 0; i < C::NDB; ++i) {
         const s16x8 v = v_op(i);
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][i] = mma16x16<CT>(v, p[r], acc[r][i]);
       }
-    };
-
-    // --- the stream --------------------------------------------------------
-    const int mine = cnt > stream ? (cnt - stream + streams - 1) / streams : 0;
-    const int rounds = (mine + C::NBUF - 1) / C::NBUF;
-    auto step = [&](int j) {
-      if constexpr (C::VLATE) load_v(meta[j], vr[j]);
-      compute(kr[j], vr[j], meta[j]);
-    };
+    }
+    if (KV != FA_KV_INT8 && __builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {
+      // The values that were left out, key by key.
+#pragma unroll 1
+      for (int k = 0; k < mine; ++k) {
+        Ahead x;
 #pragma unroll
-    for (int j = 0; j < C::NBUF; ++j) issue(c0 + stream + streams * j, kr[j], vr[j], meta[j]);
-    for (int g = 0; g + 1 < rounds; ++g) {
+        for (int h = 0; h < NH; ++h) {
+          x.logical[h] = logical_of(first_key(chunk(k), h));
+          x.page[h] = page_of(x.logical[h]);
+        }
+        const Meta m = describe(chunk(k), x);
+        if (!is_mixed(m)) continue;
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+          if (!((m.there >> key) & 1u)) continue;
+          int64_t off;
+          int pos;
+          float vs;
+          if constexpr (SMALL) {
+            off = far(m.voff[0], key);
+            pos = __shfl(m.key0[0], key, 64);
+            vs = __shfl(m.vs[0], key, 64);
+          } else {
+            off = (key < 16 ? m.voff[0] : m.voff[NH - 1]) + (key & 15) * a.v_stride[1];
+            pos = (key < 16 ? m.key0[0] : m.key0[NH - 1]) + (key & 15);
+            vs = key < 16 ? m.vs[0] : m.vs[NH - 1];
+          }
 #pragma unroll
-      for (int j = 0; j < C::NBUF; ++j) {
-        step(j);
-        issue(c0 + stream + streams * ((g + 1) * C::NBUF + j), kr[j], vr[j], meta[j]);
+          for (int i = 0; i < C::NDB; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const KE c = vbase[off + 16 * i + 4 * g4 + e];
+              float f;
+              if constexpr (C::KV8) f = (c & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+              else f = Elem<CT>::to_f(c);
+              if (f - f == 0.f) continue;
+#pragma unroll
+              for (int r = 0; r < R; ++r)
+                if (pos <= klim[r]) acc[r][i][e] += f * vs;
+            }
+        }
       }
     }
-    if (rounds > 0) {
-#pragma unroll
-      for (int j = 0; j < C::NBUF; ++j)
-        if ((rounds - 1) * C::NBUF + j < mine) step(j);
-    }
 
-    // --- the waves of a head -------------------------------------------------
+    // --- the waves' sums: out, or a partial ----------------------------------
     const float vscale = C::KV8 ? __uint_as_float(vref) : 1.f;
+    float* const so = reinterpret_cast<float*>(smem);
+    float* const sm = so + C::NW * C::RB * C::OLD;
+    float* const sl = sm + C::NW * C::RB;
+    __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       l_i[r] += __shfl_xor(l_i[r], 16, 64);
       l_i[r] += __shfl_xor(l_i[r], 32, 64);
-      if constexpr (C::KV8) {
+      const int row = wave * C::RB + 16 * r + l16;
+      if (16 * r + l16 < w.rb_rows) {
+        float* const st = so + row * C::OLD + 4 * g4;
 #pragma unroll
-        for (int i = 0; i < C::NDB; ++i) acc[r][i] *= vscale;
+        for (int i = 0; i < C::NDB; ++i) *reinterpret_cast<f32x4a*>(st + 16 * i) = acc[r][i] * vscale;
+        if (g4 == 0) {
+          sm[row] = m_i[r];
+          sl[row] = l_i[r];
+        }
       }
     }
-    float* const states = reinterpret_cast<float*>(smem);
     __syncthreads();
-    for (int half = streams >> 1; half > 0; half >>= 1) {
-      if (stream >= half && stream < 2 * half) {
-        float* const st = states + (int64_t)((stream - half) * hpw + hw) * R * C::STATE * 64 + lane;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-#pragma unroll
-          for (int i = 0; i < C::NDB; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st[(r * C::STATE + 4 * i + e) * 64] = acc[r][i][e];
-          st[(r * C::STATE + 4 * C::NDB) * 64] = m_i[r];
-          st[(r * C::STATE + 4 * C::NDB + 1) * 64] = l_i[r];
-        }
-      }
-      __syncthreads();
-      if (stream < half) {
-        const float* const st = states + (int64_t)(stream * hpw + hw) * R * C::STATE * 64 + lane;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float m2 = st[(r * C::STATE + 4 * C::NDB) * 64], l2 = st[(r * C::STATE + 4 * C::NDB + 1) * 64];
-          const float now = fmaxf(m_i[r], m2);
-          const float f1 = __builtin_amdgcn_exp2f(m_i[r] - now), f2 = __builtin_amdgcn_exp2f(m2 - now);
-          m_i[r] = now;
-          l_i[r] = l_i[r] * f1 + l2 * f2;
-#pragma unroll
-          for (int i = 0; i < C::NDB; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][i][e] = acc[r][i][e] * f1 + st[(r * C::STATE + 4 * i + e) * 64] * f2;
-        }
-      }
-      __syncthreads();
-    }
-
-    // --- out, or a partial -----------------------------------------------------
     const bool complete = cnt == all;
-    if (stream == 0) {
+    const int here = min(w.rb_rows, rows - w.rb * C::RB);
+    const int64_t part = partial_row(a, 2 * w.share + (c0 == 0 ? 1 : 0), hk, w.rb, w.nrb, w.rb_rows);
+    for (int i = tid; i < here * (D / 4); i += C::NT) {
+      const int d = i % (D / 4) * 4, r = i / (D / 4);
+      float M = sm[r];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int row = rb * RB + 16 * r + l16;
-        if (row >= rows) continue;
-        const int g = row / a.seqlen_q, mq = row - g * a.seqlen_q;
-        if (complete) {
-          const float inv = l_i[r] == 0.f ? 0.f : 1.f / l_i[r];
-          uint16_t* const op = reinterpret_cast<uint16_t*>(a.out) + b * a.out_stride[0] +
-                               (hk * group + g) * a.out_stride[1] + mq * a.out_stride[2] + 4 * g4;
+      for (int v = 1; v < C::NW; ++v) M = fmaxf(M, sm[v * C::RB + r]);
+      float L = 0.f;
+      f32x4a o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < C::NDB; ++i) {
-            s16x4 o;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (short)to_out(a, acc[r][i][e] * inv);
-            *reinterpret_cast<s16x4*>(op + 16 * i) = o;
-          }
-        } else {
-          const int64_t at_row = (((int64_t)(2 * share + (c0 == 0 ? 1 : 0)) * a.heads_kv + hk) * nrb + rb) * rb_rows +
-                                 16 * r + l16;
-          float* const po = a.ws_o + at_row * D + 4 * g4;
-          float* const pm = a.ws_ml + 2 * at_row;
-          if (a.tickets) {
-            // Written through to where every XCD sees it (the L2s are not
-            // coherent with each other).
-#pragma unroll
-            for (int i = 0; i < C::NDB; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                __hip_atomic_store(po + 16 * i + e, acc[r][i][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (g4 == 0) {
-              __hip_atomic_store(pm, m_i[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-              __hip_atomic_store(pm + 1, l_i[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < C::NDB; ++i) *reinterpret_cast<f32x4a*>(po + 16 * i) = acc[r][i];
-            if (g4 == 0) {
-              pm[0] = m_i[r];
-              pm[1] = l_i[r];
-            }
-          }
+      for (int v = 0; v < C::NW; ++v) {
+        const float f = __builtin_amdgcn_exp2f(sm[v * C::RB + r] - M);
+        L += sl[v * C::RB + r] * f;
+        o += *reinterpret_cast<const f32x4a*>(so + (v * C::RB + r) * C::OLD + d) * f;
+      }
+      if (complete) {
+        store_out(a, b, hk, w.rb * C::RB + r, d, o * (L == 0.f ? 0.f : 1.f / L));
+      } else if (a.tickets) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rsrc_of(a.ws_o), (int)(((part + r) * D + d) * 4), 0, kAgent);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, rsrc_of(a.ws_ml), (int)((part + r) * 8), 0, kAgent);
+      } else {
+        *reinterpret_cast<f32x4a*>(a.ws_o + (part + r) * D + d) = o;
+        if (d == 0) {
+          a.ws_ml[2 * (part + r)] = M;
+          a.ws_ml[2 * (part + r) + 1] = L;
         }
       }
     }
-    if (!complete && a.tickets) {
-      // The stores are acknowledged (vmcnt 0) before the workgroup's ticket;
-      // no workgroup waits for another.
-      int* const flag = reinterpret_cast<int*>(smem + C::LDS_BYTES - 16);
-      wait_vm_all();
-      __syncthreads();
-      const int j0 = cut.owner(b_begin), j1 = cut.owner(b_begin + all - 1);
-      if (tid == 0) {
-        uint32_t* const t = a.tickets + ((int64_t)b * nhg + hg) * nrb + rb;
-        const bool last = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(j1 - j0);
-        if (last) __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = last;
-      }
-      __syncthreads();
-      const int last = *flag;
-      if (last) merge_partials<D, C::NT, true>(a, b, hg, rb, nrb, rb_rows, j0, j1, tid);
-      __syncthreads();
-    }
+    if (!complete && a.tickets)
+      arrive<D, C::NT>(a, w, cut, b, b_begin, all, reinterpret_cast<int*>(smem + C::LDS_BYTES - 16), tid);
+    __syncthreads();  // the next sequence's tiles
     at += cnt;
     b_begin += all;
     ++b;
   }
 }
 
-// The merge as a launch of its own: grid (head groups * row blocks, batch).
-template <typename Tag, int KV, int D, int R, bool SMALL>
+// The merge as a launch of its own: grid (KV heads * row blocks, batch).
+// LEAST: the fewest chunks of a share, as in the kernel that wrote the partials.
+template <int D, int RB, int LEAST>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
-  using C = AttnCfg<Tag, KV, D, R, SMALL>;
-  constexpr int RB = 16 * R;
-  const int rows = a.heads_q / a.heads_kv * a.seqlen_q, nrb = (rows + RB - 1) / RB, rb_rows = min(RB, rows);
-  const int nhg = a.heads_kv >> a.head_shift, hg = blockIdx.x % nhg, rb = blockIdx.x / nhg, lane = threadIdx.x & 63;
-  const PagedWork work{a, rb_rows, rb};
-  const Shares cut = work.shares(lane, 2 * (C::NW >> a.head_shift));
+  const int lane = threadIdx.x & 63, b = blockIdx.y;
+  const SharePlace w(a, RB);
+  const PagedWork work{a, w.rb_rows, w.rb};
+  const Shares cut = work.shares(lane, LEAST);
   int begin = 0;
-  const int b = blockIdx.y;
   for (int b0 = 0; b0 < b; b0 += 64) begin += b0 + lane < b ? work.chunks(b0 + lane) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) begin += __shfl_xor(begin, o, 64);
   const int j0 = cut.owner(begin), j1 = cut.owner(begin + work.chunks(b) - 1);
-  if (j0 != j1) merge_partials<D, 256, false>(a, b, hg, rb, nrb, rb_rows, j0, j1, threadIdx.x);
+  if (j0 != j1) merge_partials<D, 256, false>(a, b, w.hk, w.rb, w.nrb, w.rb_rows, j0, j1, threadIdx.x);
 }
 
 }  // namespace fa

@@ -39,6 +39,8 @@
 #include <atomic>
 #include <cstring>
 #include <initializer_list>
+#include <map>
+#include <mutex>
 #include <optional>
 #include <tuple>
 
@@ -585,9 +587,15 @@ int32_t to_int32(int64_t n, const char* what) {
   return (int32_t)n;
 }
 
-// The tensor is written as it is: rows of 16-byte pieces, no copy.
-void check_in_place(const Tensor& t, const char* what) {
-  TORCH_CHECK(kernel_ready(t).is_same(t), "fa_mi355x: ", what, " needs a unit last stride and 16-byte aligned rows");
+// The tensor is written as it is: no element twice and, for `rows`, in
+// 16-byte pieces.
+void check_in_place(const Tensor& t, const char* what, bool rows = true) {
+  bool ok = !rows || ((t.stride(-1) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+  for (int64_t i = 0; ok && i < t.dim(); ++i)
+    if (t.size(i) > 1 && (t.stride(i) == 0 || (rows && i + 1 < t.dim() && (t.stride(i) * t.element_size()) % 16 != 0)))
+      ok = false;
+  TORCH_CHECK(ok, "fa_mi355x: ", what, " is written in place: it must not be expanded, and rows need a unit last stride ",
+              "and 16-byte alignment");
 }
 
 int kv_format_of(const Tensor& cache, const Tensor& like) {
@@ -619,6 +627,7 @@ std::tuple<Tensor, Tensor, Tensor> paged_allocate_op(const Tensor& block_table, 
   TORCH_CHECK(block_table.is_cuda() && block_table.dim() == 2, "fa_mi355x: block_table must be a 2-D GPU tensor");
   const int64_t batch = block_table.size(0);
   check_int32(block_table, block_table, block_table.sizes(), "block_table");
+  check_in_place(block_table, "block_table", false);
   check_int32(context_lens, block_table, {batch}, "context_lens");
   check_int32(new_lens, block_table, {batch}, "new_lens");
   TORCH_CHECK(free_blocks.dim() == 1, "fa_mi355x: free_blocks must be 1-D");
@@ -668,7 +677,13 @@ void paged_append_op(const Tensor& key, const Tensor& value, const Tensor& k_cac
                   slots.size(0) == key.size(0),
               "fa_mi355x: slot_mapping must be int64 (tokens,) on key's device");
   const int format = kv_format_of(k_cache, key);
-  if (format != FA_KV_SAME) check_scales(k_scale, v_scale, k_cache);
+  if (format != FA_KV_SAME) {
+    check_scales(k_scale, v_scale, k_cache);
+    check_in_place(*k_scale, "k_scale", false);
+    check_in_place(*v_scale, "v_scale", false);
+  } else {
+    TORCH_CHECK(!k_scale.has_value() && !v_scale.has_value(), "fa_mi355x: scales are for 8-bit caches");
+  }
   check_in_place(k_cache, "k_cache");
   check_in_place(v_cache, "v_cache");
   if (key_bounds.has_value()) {
@@ -712,11 +727,12 @@ void paged_append_op(const Tensor& key, const Tensor& value, const Tensor& k_cac
   check_status(fa_paged_append(&p, stream_of(key)), "fa_paged_append");
 }
 
-Tensor paged_select_op(const Tensor& query, const Tensor& key_bounds, const Tensor& block_table,
+Tensor paged_select_op(const Tensor& query_in, const Tensor& key_bounds, const Tensor& block_table,
                        const Tensor& context_lens, int64_t num_selected, int64_t block_size, int64_t keep_first,
                        int64_t keep_last) {
-  check_16bit(query, "query");
-  TORCH_CHECK(query.dim() == 4, "fa_mi355x: query must be (batch, heads, rows, head_dim)");
+  check_16bit(query_in, "query");
+  TORCH_CHECK(query_in.dim() == 3 || query_in.dim() == 4, "fa_mi355x: query must be (batch, heads[, rows], head_dim)");
+  const Tensor query = query_in.dim() == 3 ? query_in.unsqueeze(2) : query_in;
   TORCH_CHECK(key_bounds.device() == query.device() && key_bounds.scalar_type() == query.scalar_type() &&
                   key_bounds.dim() == 4 && key_bounds.size(2) == 2 && key_bounds.size(3) == query.size(3),
               "fa_mi355x: key_bounds must be (blocks, heads_kv, 2, head_dim) in the query's dtype, on its device");
@@ -757,13 +773,34 @@ Tensor paged_select_op(const Tensor& query, const Tensor& key_bounds, const Tens
   return index;
 }
 
-Tensor decode_paged_blocks_op(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+// Arrival counters of decode_paged_blocks: zero between calls, one buffer for
+// each (device, stream), since calls on a stream follow each other.  None
+// under graph capture: replays of two graphs may overlap, on any streams.
+Tensor stream_tickets(const Tensor& query, int64_t need) {
+  const auto stream = c10::hip::getCurrentHIPStream(query.device().index());
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess || capture != hipStreamCaptureStatusNone)
+    return Tensor();
+  static std::mutex mu;
+  // (Never destroyed: at exit the allocator may be gone first.)
+  static auto* const buffers = new std::map<std::pair<int, hipStream_t>, Tensor>();
+  std::lock_guard<std::mutex> lock(mu);
+  Tensor& buf = (*buffers)[{(int)query.device().index(), stream.stream()}];
+  if (!buf.defined() || buf.numel() < need)
+    buf = at::zeros({std::max<int64_t>(need, buf.defined() ? 2 * buf.numel() : 1024)}, query.options().dtype(at::kInt));
+  return buf;
+}
+
+Tensor decode_paged_blocks_op(const Tensor& query_in, const Tensor& k_cache, const Tensor& v_cache,
                               const Tensor& block_table, const Tensor& context_lens, const OptTensor& k_scale,
                               const OptTensor& v_scale, const OptTensor& block_index, bool causal, double scale,
-                              int64_t shares, const OptTensor& tickets) {
-  check_16bit(query, "query");
+                              int64_t shares, bool fused_merge) {
+  check_16bit(query_in, "query");
+  TORCH_CHECK(query_in.dim() == 3 || query_in.dim() == 4, "fa_mi355x: query must be (batch, heads[, rows], head_dim)");
+  const Tensor query = query_in.dim() == 3 ? query_in.unsqueeze(2) : query_in;
   const int format = kv_format_of(k_cache, query);
-  TORCH_CHECK(query.dim() == 4, "fa_mi355x: query must be (batch, heads, rows, head_dim)");
+  if (format == FA_KV_SAME)
+    TORCH_CHECK(!k_scale.has_value() && !v_scale.has_value(), "fa_mi355x: scales are for 8-bit caches");
   for (const Tensor* t : {&k_cache, &v_cache})
     TORCH_CHECK(t->device() == query.device() && t->dim() == 4 && t->sizes() == k_cache.sizes() &&
                     t->scalar_type() == k_cache.scalar_type() && t->size(3) == query.size(3),
@@ -777,7 +814,6 @@ Tensor decode_paged_blocks_op(const Tensor& query, const Tensor& k_cache, const 
     TORCH_CHECK(block_index->dim() == 3, "fa_mi355x: block_index must be 3-D");
     check_int32(*block_index, query, {query.size(0), k_cache.size(2), block_index->size(2)}, "block_index");
   }
-  check_tickets(tickets, query);
   c10::DeviceGuard guard(query.device());
   const Tensor q = kernel_ready(query), k = kernel_ready(k_cache), v = kernel_ready(v_cache);
   const Tensor out = at::empty(q.sizes(), q.options());
@@ -822,9 +858,11 @@ Tensor decode_paged_blocks_op(const Tensor& query, const Tensor& k_cache, const 
   p.shares = to_int32(shares, "shares");
   const Tensor ws = at::empty({(int64_t)fa_paged_blocks_workspace_bytes(&p)}, q.options().dtype(at::kByte));
   p.workspace = ws.data_ptr();
-  if (tickets.has_value()) p.tickets = reinterpret_cast<uint32_t*>(tickets->data_ptr<int32_t>());
+  Tensor tickets;
+  if (fused_merge) tickets = stream_tickets(query, (int64_t)fa_decode_ticket_count(p.batch, p.heads_q, p.seqlen_q));
+  if (tickets.defined()) p.tickets = reinterpret_cast<uint32_t*>(tickets.data_ptr<int32_t>());
   check_status(fa_decode_paged_blocks(&p, stream_of(query)), "fa_decode_paged_blocks");
-  return out;
+  return query_in.dim() == 3 ? out.squeeze(2) : out;
 }
 
 // Inside a torch.func transform.  Decode has no rule for any of them, and a
@@ -873,7 +911,7 @@ TORCH_LIBRARY(fa_mi355x, m) {
         "int block_size, int keep_first, int keep_last) -> Tensor");
   m.def("decode_paged_blocks(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, "
         "Tensor? k_scale, Tensor? v_scale, Tensor? block_index, bool causal, float scale, int shares, "
-        "Tensor(a!)? tickets) -> Tensor");
+        "bool fused_merge) -> Tensor");
   m.def("set_ds_scratch_limit(int bytes) -> int", &set_ds_scratch_limit);
   m.def("ds_scratch_limit() -> int", &ds_scratch_limit);
 }

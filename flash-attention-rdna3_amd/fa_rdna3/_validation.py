@@ -224,13 +224,15 @@ EIGHT_BIT_DTYPES = (torch.float8_e4m3fn, torch.int8)
 EIGHT_BIT_HEAD_DIMS = (32, 64, 128, 256, 512)
 
 
-def _require_count(name, value, least):
+def validate_count(name, value, least):
+    """A 32-bit whole number of at least `least`."""
     if isinstance(value, bool) or not isinstance(value, Integral) or not least <= value < 2 ** 31:
         raise ValueError(f"{name} must be an integer of at least {least}")
 
 
-def _require_block_size(block_size):
-    _require_count("block_size", block_size, 1)
+def validate_block_size(block_size):
+    """Tokens of a paged cache's block."""
+    validate_count("block_size", block_size, 1)
     if block_size > 256 or block_size & (block_size - 1):
         raise ValueError("paged cache block size must be a power of two up to 256")
 
@@ -255,7 +257,7 @@ def _require_writable(name, tensor, rows=False):
         raise ValueError(f"{name} must have a unit last stride and 16-byte aligned rows to be updated in place")
 
 
-def validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, free_head, block_size, num_tokens):
+def validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, free_head):
     _require_tensor("block_table", block_table)
     device = block_table.device
     _require_like("block_table", block_table, torch.int32, (None, None), device)
@@ -267,8 +269,6 @@ def validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, f
     _require_like("free_blocks", free_blocks, torch.int32, (None,), device)
     if free_head is not None:
         _require_like("free_head", free_head, torch.int32, (1,), device)
-    _require_block_size(block_size)
-    _require_count("num_tokens", num_tokens, 0)
     _require_writable("block_table", block_table)
     _require_platform(device)
 
@@ -287,7 +287,7 @@ def validate_append_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale, 
     _require_like("v_cache", v_cache, k_cache.dtype, k_cache.shape, device)
     if min(heads, dim, k_cache.shape[0]) <= 0:
         raise ValueError("kv_heads, head_dim and blocks must be positive")
-    _require_block_size(k_cache.shape[1])
+    validate_block_size(k_cache.shape[1])
     eight = k_cache.dtype in EIGHT_BIT_DTYPES
     if dim not in (EIGHT_BIT_HEAD_DIMS if eight else SUPPORTED_HEAD_DIMS):
         raise ValueError(f"head_dim {dim} is not supported by a paged cache of {str(k_cache.dtype).removeprefix('torch.')}")
@@ -306,8 +306,7 @@ def validate_append_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale, 
     _require_platform(device)
 
 
-def validate_select_inputs(query, key_bounds, block_table, context_lens, num_selected, block_size, keep_first,
-                           keep_last):
+def validate_select_inputs(query, key_bounds, block_table, context_lens):
     _require_tensor("query", query)
     device = query.device
     if query.dim() not in (3, 4) or query.dtype not in LOW_PRECISION_DTYPES:
@@ -324,12 +323,6 @@ def validate_select_inputs(query, key_bounds, block_table, context_lens, num_sel
     if block_table.shape[1] <= 0:
         raise ValueError("block_table must contain at least one logical block")
     _require_like("context_lens", context_lens, torch.int32, (batch,), device)
-    _require_block_size(block_size)
-    _require_count("num_selected", num_selected, 1)
-    _require_count("keep_first", keep_first, 0)
-    _require_count("keep_last", keep_last, 0)
-    if keep_first + keep_last > num_selected:
-        raise ValueError("keep_first + keep_last must not exceed num_selected")
     _require_platform(device)
 
 
@@ -348,7 +341,7 @@ def validate_paged_blocks_inputs(query, k_cache, v_cache, block_table, context_l
     if query.shape[-1] not in EIGHT_BIT_HEAD_DIMS:
         raise ValueError("block scales and block_index need head_dim 32, 64, 128, 256 or 512")
     if k_cache.dim() == 4:
-        _require_block_size(k_cache.shape[1])
+        validate_block_size(k_cache.shape[1])
         if eight:
             for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
                 _require_like(name, scale, torch.float32, (k_cache.shape[0], k_cache.shape[2]), query.device)

@@ -721,9 +721,8 @@ def flash_attention_decode_paged(query, k_cache, v_cache, block_table, context_l
     """
     if _wants_blocks(k_cache, k_scale, v_scale, block_index):
         _require_tensor_dims(query, 3)
-        out = _paged_blocks(query.unsqueeze(2), k_cache, v_cache, block_table, context_lens, softmax_scale,
-                            max_context_len, num_splits, False, k_scale, v_scale, block_index)
-        return out.squeeze(2)
+        return _paged_blocks(query, k_cache, v_cache, block_table, context_lens, softmax_scale, max_context_len,
+                             num_splits, False, k_scale, v_scale, block_index)
     fp8 = _validate_paged(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale)
     validate_inference_only(query, k_cache, v_cache)
     validate_softmax_scale(softmax_scale)
@@ -772,25 +771,28 @@ def _require_tensor_dims(query, dims):
 
 def _paged_blocks(query, k_cache, v_cache, block_table, context_lens, softmax_scale, max_context_len, num_splits,
                   causal, k_scale, v_scale, block_index):
-    """Checks and launch of a (batch, q_heads, Sq, head_dim) query over block
-    scales or listed blocks."""
-    if isinstance(k_cache, torch.Tensor) and k_cache.dtype == torch.float8_e4m3fn and k_cache.dim() == 4:
-        if not isinstance(k_scale, torch.Tensor) and not isinstance(v_scale, torch.Tensor):
+    """Checks and launch of a (batch, q_heads[, Sq], head_dim) query over
+    block scales or listed blocks."""
+    if not isinstance(k_scale, torch.Tensor) and not isinstance(v_scale, torch.Tensor):
+        if isinstance(k_cache, torch.Tensor) and k_cache.dtype == torch.float8_e4m3fn and k_cache.dim() == 4:
             # Listed blocks of a cache with one scale for all of them.
             _check_fp8_pair(v_cache, k_scale, v_scale)
             shape = (k_cache.shape[0], k_cache.shape[2])
             k_scale, v_scale = (torch.full((1, 1), 1.0 if s is None else float(s), device=k_cache.device).expand(shape)
                                 for s in (k_scale, v_scale))
-    validate_paged_blocks_inputs(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale, block_index)
-    validate_inference_only(query, k_cache, v_cache)
     validate_softmax_scale(softmax_scale)
     _paged_options(max_context_len, num_splits)
-    batch, q_heads, seqlen_q, head_dim = query.shape
-    softmax_scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
-    shares = 0 if num_splits is None else min(4096, int(num_splits) * batch)
-    return _native.ops().decode_paged_blocks(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale,
-                                             block_index, causal, softmax_scale, shares,
-                                             _native.decode_tickets(query, batch, q_heads, seqlen_q))
+    softmax_scale = 1.0 / math.sqrt(max(query.shape[-1], 1)) if softmax_scale is None else float(softmax_scale)
+    shares = 0 if num_splits is None else min(4096, int(num_splits) * max(query.shape[0], 1))
+    try:
+        validate_inference_only(query, k_cache, v_cache)
+        return _native.ops().decode_paged_blocks(query, k_cache, v_cache, block_table, context_lens, k_scale, v_scale,
+                                                 block_index, causal, softmax_scale, shares, _native.FUSED_SPLIT_MERGE)
+    except (RuntimeError, TypeError, AttributeError):
+        # The operator refuses before it launches; this finds the message.
+        validate_paged_blocks_inputs(query.unsqueeze(2) if query.dim() == 3 else query, k_cache, v_cache, block_table,
+                                     context_lens, k_scale, v_scale, block_index)
+        raise
 
 
 def _paged_options(max_context_len, num_splits):

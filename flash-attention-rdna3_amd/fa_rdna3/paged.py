@@ -12,12 +12,20 @@ serving loop over this package's paged decode is
 
 with every argument on the GPU: nothing waits for the host, and the whole step
 can be captured into a HIP graph.  All of it is inference-only.
+
+The native operators check what they are given before anything is launched; a
+call that they refuse is looked over again here, for this package's messages.
+(All the checks in Python took longer than the kernels of a small step.)
 """
+
+import torch
 
 from . import _native
 from ._validation import (
     validate_allocate_inputs,
     validate_append_inputs,
+    validate_block_size,
+    validate_count,
     validate_inference_only,
     validate_select_inputs,
 )
@@ -50,9 +58,14 @@ def paged_kvcache_allocate(block_table, context_lens, new_lens, free_blocks, *, 
         missing).  ``context_lens`` and ``free_head`` are not modified, and
         the same call again gives the same tables.
     """
-    validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, free_head, block_size, num_tokens)
-    return _native.ops().paged_allocate(block_table, context_lens, new_lens, free_blocks, free_head, int(block_size),
-                                        int(num_tokens))
+    validate_block_size(block_size)
+    validate_count("num_tokens", num_tokens, 0)
+    try:
+        return _native.ops().paged_allocate(block_table, context_lens, new_lens, free_blocks, free_head, block_size,
+                                            num_tokens)
+    except (RuntimeError, TypeError):
+        validate_allocate_inputs(block_table, context_lens, new_lens, free_blocks, free_head)
+        raise
 
 
 def paged_kvcache_append(key, value, k_cache, v_cache, slot_mapping, *, k_scale=None, v_scale=None, key_bounds=None):
@@ -82,9 +95,14 @@ def paged_kvcache_append(key, value, k_cache, v_cache, slot_mapping, *, k_scale=
     stored as the largest code and have no part in the scale; NaN stays NaN
     (int8: 0) and has no part in scale or bounds.
     """
-    validate_append_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, key_bounds)
-    validate_inference_only(*(t for t in (k_cache, v_cache, k_scale, v_scale, key_bounds) if t is not None))
-    _native.ops().paged_append(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, key_bounds)
+    for written in (k_cache, v_cache, k_scale, v_scale, key_bounds):
+        if isinstance(written, torch.Tensor):
+            validate_inference_only(written)
+    try:
+        _native.ops().paged_append(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, key_bounds)
+    except (RuntimeError, TypeError):
+        validate_append_inputs(key, value, k_cache, v_cache, slot_mapping, k_scale, v_scale, key_bounds)
+        raise
 
 
 def paged_kvcache_select(query, key_bounds, block_table, context_lens, num_selected, *, block_size, keep_first=0,
@@ -112,8 +130,16 @@ def paged_kvcache_select(query, key_bounds, block_table, context_lens, num_selec
         ``block_index`` of the paged decode.  Equal scores go to the lower
         index.
     """
-    validate_select_inputs(query, key_bounds, block_table, context_lens, num_selected, block_size, keep_first, keep_last)
-    validate_inference_only(query, key_bounds)
-    rows = query.unsqueeze(2) if query.dim() == 3 else query
-    return _native.ops().paged_select(rows, key_bounds, block_table, context_lens, int(num_selected), int(block_size),
-                                      int(keep_first), int(keep_last))
+    validate_block_size(block_size)
+    validate_count("num_selected", num_selected, 1)
+    validate_count("keep_first", keep_first, 0)
+    validate_count("keep_last", keep_last, 0)
+    if keep_first + keep_last > num_selected:
+        raise ValueError("keep_first + keep_last must not exceed num_selected")
+    try:
+        validate_inference_only(query, key_bounds)
+        return _native.ops().paged_select(query, key_bounds, block_table, context_lens, num_selected, block_size,
+                                          keep_first, keep_last)
+    except (RuntimeError, TypeError, AttributeError):
+        validate_select_inputs(query, key_bounds, block_table, context_lens)
+        raise
