@@ -12,22 +12,26 @@ int log2_floor(int n) {
   return s;
 }
 
-// Row blocks of 16 that a wave holds (R): more of them share the conversion
-// and the loads of a chunk.
-int row_blocks(const fa_paged_blocks_params& p) {
-  const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
-  if (p.kv_format == FA_KV_SAME || p.head_dim > 128 || p.block_size < 16 || rows <= 16) return 1;
-  return 2;
+PageMode page_mode(const fa_paged_blocks_params& p) {
+  const int es = p.kv_format == FA_KV_SAME ? 2 : 1;
+  auto small = [](int64_t bytes) { return bytes >= 0 && bytes < (int64_t(1) << 31); };
+  const bool plain = small(p.k_stride[0] * es) && small(p.k_stride[1] * es) && small(p.v_stride[0] * es) &&
+                     small(p.v_stride[1] * es) && small(p.k_scale_stride[0]) && small(p.v_scale_stride[0]) &&
+                     small(p.block_table_stride[1]);
+  return !plain || p.block_size < 16 ? kAnyPages : p.block_size == 16 ? kTwoPages : kOnePage;
 }
 
 struct Plan {
-  int r, nrb, rb_rows, shares;
+  PageMode pages;
+  int r;  // row blocks of 16 that a wave holds: two share the loads and the conversion of a chunk
+  int nrb, rb_rows, shares;
 };
 
 Plan plan_of(const fa_paged_blocks_params& p) {
   Plan w;
-  w.r = row_blocks(p);
+  w.pages = page_mode(p);
   const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
+  w.r = p.kv_format == FA_KV_SAME || p.head_dim > 128 || w.pages == kAnyPages || rows <= 16 ? 1 : 2;
   w.nrb = (int)((rows + 16 * w.r - 1) / (16 * w.r));
   w.rb_rows = (int)std::min<int64_t>(rows, 16 * w.r);
   const int64_t columns = (int64_t)p.heads_kv * w.nrb;
@@ -40,10 +44,10 @@ int64_t partial_rows(const fa_paged_blocks_params& p, const Plan& w) {
   return 2 * (int64_t)w.shares * p.heads_kv * w.nrb * w.rb_rows;
 }
 
-template <typename Tag, int KV, int D, int R, bool SMALL>
+template <typename Tag, int KV, int D, int R, int PAGES>
 hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
-  using C = AttnCfg<Tag, KV, D, R, SMALL>;
-  auto kern = paged_attn_kernel<Tag, KV, D, R, SMALL>;
+  using C = AttnCfg<Tag, KV, D, R, PAGES>;
+  auto kern = paged_attn_kernel<Tag, KV, D, R, PAGES>;
   hipError_t e = allow_lds((const void*)kern, C::LDS_BYTES);
   if (e != hipSuccess) return e;
   const int columns = a.heads_kv * w.nrb;
@@ -57,11 +61,13 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
 
 template <typename Tag, int KV, int D>
 hipError_t run_dim(const PagedAttnArgs& a, const Plan& w, hipStream_t s) {
-  if (a.shift < 4) return run<Tag, KV, D, 1, true>(a, w, s);
+  if (w.pages == kAnyPages) return run<Tag, KV, D, 1, kAnyPages>(a, w, s);
   if constexpr (KV != FA_KV_SAME && D <= 128) {
-    if (w.r == 2) return run<Tag, KV, D, 2, false>(a, w, s);
+    if (w.r == 2 && w.pages == kOnePage) return run<Tag, KV, D, 2, kOnePage>(a, w, s);
+    if (w.r == 2) return run<Tag, KV, D, 2, kTwoPages>(a, w, s);
   }
-  return run<Tag, KV, D, 1, false>(a, w, s);
+  if (w.pages == kOnePage) return run<Tag, KV, D, 1, kOnePage>(a, w, s);
+  return run<Tag, KV, D, 1, kTwoPages>(a, w, s);
 }
 
 template <typename Tag, int KV>
@@ -95,8 +101,8 @@ hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
   for (int i = 0; i < 3; ++i) {
     a.q_stride[i] = p.q_stride[i];
     a.out_stride[i] = p.out_stride[i];
-    a.k_stride[i] = p.k_stride[i];
-    a.v_stride[i] = p.v_stride[i];
+    a.k_stride[i] = p.k_stride[i] * (p.kv_format == FA_KV_SAME ? 2 : 1);
+    a.v_stride[i] = p.v_stride[i] * (p.kv_format == FA_KV_SAME ? 2 : 1);
     a.index_stride[i] = p.block_index_stride[i];
   }
   a.table = p.block_table;

@@ -46,7 +46,7 @@ struct PagedAttnArgs {
   int64_t out_stride[3];
   const void* k;
   const void* v;
-  int64_t k_stride[3];  // block, position, head
+  int64_t k_stride[3];  // block, position, head; in bytes
   int64_t v_stride[3];
   const int32_t* table;
   int64_t table_stride[2];
@@ -68,7 +68,12 @@ struct PagedAttnArgs {
   uint32_t* tickets;
 };
 
-template <typename Tag, int KV, int D, int R, bool SMALL>
+// How a chunk finds its pages.  Strides below 2^31 bytes, one page for its 32
+// keys or one for each half: scalar loads and 32-bit products.  Else each lane
+// finds the page of a key of its own.
+enum PageMode { kOnePage, kTwoPages, kAnyPages };
+
+template <typename Tag, int KV, int D, int R, int PAGES>
 struct AttnCfg {
   static constexpr bool KV8 = KV != FA_KV_SAME;
   // Waves: two per SIMD where a chunk and the sums leave room for them.
@@ -99,22 +104,30 @@ template <> __device__ inline f32x4a mma16x16<bf16_t>(s16x8 a, s16x8 b, f32x4a c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
 }
 
-// Eight int8 codes as fp16, exactly: 1024 + (x + 128) is the fp16 number with
-// bits 0x6400 + (x + 128); subtract 1152.
+// int8 codes x as fp16 1152 + x (bits 0x6400 + 128 + x).  In Q K^T the 1152
+// times the row's sum is taken off by the accumulator's first value: the sums
+// then pass through values of up to ten times those of |q| |k|, in fp32 still
+// 2^-20 of them.  (Not for V, where the sum runs over all the keys.)
+constexpr float kInt8Offset = 1152.f;
+template <bool OFFSET>
 __device__ inline s16x8 int8x8_to_f16(u32x2 r) {
   uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t u = r[i] ^ 0x80808080u;
-    const h16x2 c = {(_Float16)1152.f, (_Float16)1152.f};
-    o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - c);
-    o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - c);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = r[i / 2] ^ 0x80808080u;
+    o[i] = __builtin_amdgcn_perm(0x64646464u, u, i % 2 ? 0x04030402u : 0x04010400u);
+    if constexpr (!OFFSET) {
+      const h16x2 c = {(_Float16)kInt8Offset, (_Float16)kInt8Offset};
+      const h16x2 x = __builtin_bit_cast(h16x2, o[i]) - c;
+      o[i] = __builtin_bit_cast(uint32_t, x);
+    }
   }
   return __builtin_bit_cast(s16x8, u32x4{o[0], o[1], o[2], o[3]});
 }
 
-template <int KV> __device__ inline s16x8 codes_to_f16(u32x2 r) {
-  if constexpr (KV == FA_KV_INT8) return int8x8_to_f16(r);
+// Eight codes as fp16, exactly; for K, int8 ones with the offset.
+template <int KV, bool K> __device__ inline s16x8 codes_to_f16(u32x2 r) {
+  if constexpr (KV == FA_KV_INT8) return int8x8_to_f16<K>(r);
   else return fp8x8_to_op<f16_t>(r);
 }
 
@@ -323,12 +336,14 @@ __device__ inline float bf16_row_top(const s16x8 (&q)[N]) {
   return top;
 }
 
-template <typename Tag, int KV, int D, int R, bool SMALL>
-__global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_attn_kernel(PagedAttnArgs a) {
-  using C = AttnCfg<Tag, KV, D, R, SMALL>;
+template <typename Tag, int KV, int D, int R, int PAGES>
+__global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_attn_kernel(PagedAttnArgs a) {
+  using C = AttnCfg<Tag, KV, D, R, PAGES>;
   using CT = typename std::conditional<C::KV8, f16_t, Tag>::type;  // type of the products
-  using KE = typename std::conditional<C::KV8, uint8_t, uint16_t>::type;
   using KRaw = typename std::conditional<C::KREGS == 2, u32x2, u32x4>::type;
+  constexpr bool ANY = PAGES == kAnyPages;
+  constexpr int NH = PAGES == kTwoPages ? 2 : 1;  // pages a chunk is described by
+  constexpr int ES = C::KV8 ? 1 : 2;              // bytes of an element
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -343,12 +358,22 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
   int b, b_begin;
   work.find(begin, lane, b, b_begin);
 
-  const KE* const kbase = reinterpret_cast<const KE*>(a.k) + hk * a.k_stride[2];
-  const KE* const vbase = reinterpret_cast<const KE*>(a.v) + hk * a.v_stride[2];
+  // This lane's K row of a half (l16) and V row of a chunk's first piece.
+  typedef const unsigned char* bytes;
+  const bytes kbase = static_cast<bytes>(a.k) + hk * a.k_stride[2], vbase = static_cast<bytes>(a.v) + hk * a.v_stride[2];
+  const bytes klane = kbase + (ANY ? 0 : l16 * a.k_stride[1]) + (C::PAIR || !C::KV8 ? 16 : 8) * g4;
+  constexpr int RPI = 64 / C::PPR;  // V rows of one load
+  const bytes vlane = vbase + (ANY ? 0 : (lane / C::PPR & 15) * a.v_stride[1]) + lane % C::PPR * 16;
   uint16_t* const tile = reinterpret_cast<uint16_t*>(smem) + wave * (32 * D);
   const int mask = (1 << a.shift) - 1;
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   typedef const __attribute__((address_space(4))) float const_f32;
+  // Strides of the scalar paths (below 2^31).
+  const uint32_t k0 = (uint32_t)a.k_stride[0], k1 = (uint32_t)a.k_stride[1];
+  const uint32_t v0 = (uint32_t)a.v_stride[0], v1 = (uint32_t)a.v_stride[1];
+  const uint32_t ks0 = (uint32_t)a.ks_stride[0], vs0 = (uint32_t)a.vs_stride[0], t1 = (uint32_t)a.table_stride[1];
+  const float* const ks_head = a.ks ? a.ks + hk * a.ks_stride[1] : nullptr;
+  const float* const vs_head = a.vs ? a.vs + hk * a.vs_stride[1] : nullptr;
 
   for (int at = begin; at < end;) {
     const int len = work.length(b), all = work.chunks(b);
@@ -360,33 +385,31 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
 
     // --- what a chunk's keys are ------------------------------------------
     // Two steps ahead of its use a chunk is known by its logical blocks, one
-    // step by its pages.  Pages of 16 keys or more: one each for keys 0 .. 15
-    // and 16 .. 31, scalar loads.  Smaller pages: lane l describes key l % 32.
-    constexpr int NH = SMALL ? 1 : 2;
+    // step by its pages.  kAnyPages: lane l describes key l % 32.
     struct Ahead {
       int logical[NH], page[NH];
     };
     struct Meta {
       uint32_t there;      // bit k: key k of the chunk is one of the sequence's
-      int key0[NH];        // position of the half's first key, or of the lane's
+      int key0[NH];        // position of the page's first key here, or of the lane's
       float ks[NH], vs[NH];
       int64_t koff[NH], voff[NH];
     };
-    auto first_key = [&](int c, int h) { return 32 * c + (SMALL ? lane & 31 : 16 * h); };
+    auto first_key = [&](int c, int h) { return 32 * c + (ANY ? lane & 31 : 16 * h); };
     // The logical block of the listed block that holds key n of the list.
     auto logical_of = [&](int n) {
       const int at_list = n >> a.shift;
       if (!index) return at_list;
       const int64_t i = (int64_t)min(at_list, listed - 1) * a.index_stride[2];
       int l;
-      if constexpr (SMALL) l = index[i];
+      if constexpr (ANY) l = index[i];
       else l = ((const_i32*)index)[i];
       return at_list < listed ? l : -1;
     };
     auto page_of = [&](int logical) {
-      const int64_t i = (int64_t)min(max(logical, 0), a.max_blocks - 1) * a.table_stride[1];
-      if constexpr (SMALL) return table[i];
-      else return ((const_i32*)table)[i];
+      const int l = min(max(logical, 0), a.max_blocks - 1);
+      if constexpr (ANY) return table[l * a.table_stride[1]];
+      else return ((const_i32*)table)[(uint64_t)(uint32_t)l * t1];
     };
     auto describe = [&](int c, const Ahead& x) -> Meta {
       Meta m;
@@ -394,25 +417,28 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const int inside = first_key(c, h) & mask;
-        const bool ok = x.logical[h] >= 0 && x.logical[h] < blocks && x.page[h] >= 0 && x.page[h] < a.num_blocks;
+        const bool ok = (uint32_t)x.logical[h] < (uint32_t)blocks && (uint32_t)x.page[h] < (uint32_t)a.num_blocks;
         const int page = ok ? x.page[h] : 0;
-        m.key0[h] = ok ? (x.logical[h] << a.shift) + inside : 0;
-        m.koff[h] = page * a.k_stride[0] + inside * a.k_stride[1];
-        m.voff[h] = page * a.v_stride[0] + inside * a.v_stride[1];
-        m.ks[h] = m.vs[h] = 1.f;
+        m.key0[h] = (x.logical[h] << a.shift) + inside;
         const int here = ok ? len - m.key0[h] : 0;  // keys from this one on
-        if constexpr (SMALL) {
+        m.ks[h] = m.vs[h] = 1.f;
+        if constexpr (ANY) {
+          m.koff[h] = page * a.k_stride[0] + inside * a.k_stride[1];
+          m.voff[h] = page * a.v_stride[0] + inside * a.v_stride[1];
           if constexpr (C::KV8) {
-            if (a.ks) m.ks[h] = a.ks[page * a.ks_stride[0] + hk * a.ks_stride[1]];
-            if (a.vs) m.vs[h] = a.vs[page * a.vs_stride[0] + hk * a.vs_stride[1]];
+            if (a.ks) m.ks[h] = ks_head[page * a.ks_stride[0]];
+            if (a.vs) m.vs[h] = vs_head[page * a.vs_stride[0]];
           }
           m.there = (uint32_t)__builtin_amdgcn_ballot_w64(here > 0);
         } else {
+          m.koff[h] = (int64_t)((uint64_t)(uint32_t)page * k0 + (uint64_t)(uint32_t)inside * k1);
+          m.voff[h] = (int64_t)((uint64_t)(uint32_t)page * v0 + (uint64_t)(uint32_t)inside * v1);
           if constexpr (C::KV8) {
-            if (a.ks) m.ks[h] = ((const_f32*)a.ks)[page * a.ks_stride[0] + hk * a.ks_stride[1]];
-            if (a.vs) m.vs[h] = ((const_f32*)a.vs)[page * a.vs_stride[0] + hk * a.vs_stride[1]];
+            if (a.ks) m.ks[h] = ((const_f32*)ks_head)[(uint64_t)(uint32_t)page * ks0];
+            if (a.vs) m.vs[h] = ((const_f32*)vs_head)[(uint64_t)(uint32_t)page * vs0];
           }
-          m.there |= (here > 0 ? 0xFFFFu >> (16 - min(here, 16)) : 0u) << (16 * h);
+          constexpr int W = NH == 2 ? 16 : 32;
+          m.there |= (here > 0 ? 0xFFFFFFFFu >> (32 - min(here, W)) : 0u) << (16 * h);
         }
         m.vs[h] = here > 0 ? m.vs[h] : 0.f;
       }
@@ -427,26 +453,30 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
     auto load_k = [&](const Meta& m) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int64_t off;
-        if constexpr (SMALL) off = far(m.koff[0], 16 * h + l16);
-        else off = m.koff[h] + l16 * a.k_stride[1];
+        bytes p;
+        if constexpr (ANY) p = klane + far(m.koff[0], 16 * h + l16);
+        else p = klane + (NH == 2 ? m.koff[h] : m.koff[0] + 16 * h * (int64_t)k1);
 #pragma unroll
-        for (int s = 0; s < C::KN; ++s)
-          kd[h][s] = *reinterpret_cast<const KRaw*>(kbase + off + (C::PAIR ? 64 * s + 16 * g4 : 32 * s + 8 * g4));
+        for (int s = 0; s < C::KN; ++s) kd[h][s] = *reinterpret_cast<const KRaw*>(p + (C::PAIR || !C::KV8 ? 64 : 32) * s);
       }
     };
     auto load_v = [&](const Meta& m) {
 #pragma unroll
       for (int i = 0; i < C::VN; ++i) {
-        const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
-        int64_t off;
-        if constexpr (SMALL) off = far(m.voff[0], row);
-        else off = (row < 16 ? m.voff[0] : m.voff[1]) + (row & 15) * a.v_stride[1];
-        vd[i] = *reinterpret_cast<const u32x4*>(vbase + off + col);
+        bytes p;
+        if constexpr (ANY) {
+          p = vlane + far(m.voff[0], (64 * i + lane) / C::PPR);
+        } else if constexpr (RPI > 16) {  // both halves in one load
+          p = vlane + (lane < 32 ? m.voff[0] : NH == 2 ? m.voff[NH - 1] : m.voff[0] + 16 * (int64_t)v1);
+        } else {
+          constexpr int HALF = 16 / (RPI > 16 ? 16 : RPI);  // loads of 16 rows
+          p = vlane + (NH == 2 ? m.voff[i / HALF] + i % HALF * RPI * (int64_t)v1 : m.voff[0] + i * RPI * (int64_t)v1);
+        }
+        vd[i] = *reinterpret_cast<const u32x4*>(p);
       }
     };
     const int mine = cnt > wave ? (cnt - wave + C::NW - 1) / C::NW : 0;
-    auto chunk = [&](int k) { return c0 + wave + C::NW * min(k, max(mine - 1, 0)); };
+    auto chunk = [&](int k) { return min(c0 + wave + C::NW * k, c0 + cnt - 1); };
     Ahead next, later;  // of the chunks k + 1 and k + 2
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
@@ -484,6 +514,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
     next = later;
 #pragma unroll
     for (int h = 0; h < NH; ++h) later.logical[h] = logical_of(first_key(chunk(2), h));
+    float zero[R];  // first value of Q K^T's sums
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       qscale[r] = a.scale_log2;
@@ -492,6 +523,15 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         qscale[r] *= bf16_row_to_f16(q[r], top);
+      }
+      zero[r] = 0.f;
+      if constexpr (KV == FA_KV_INT8) {
+        const short c = (short)Elem<f16_t>::from_f(-kInt8Offset);
+        const s16x8 off = {c, c, c, c, c, c, c, c};
+        f32x4a x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < C::NSTEP; ++s) x = mma16x16<f16_t>(off, q[r][s], x);
+        zero[r] = x[0];
       }
     }
 
@@ -510,9 +550,10 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
     constexpr uint32_t ABS = C::KV8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
     constexpr uint32_t UP = C::KV8 ? 0x01010101u : std::is_same<CT, bf16_t>::value ? 0x00800080u : 0x04000400u;
     uint32_t odd = 0;  // such a value was left out
+    // Some rows see keys of the chunk that others do not.
     auto is_mixed = [&](const Meta& m) {
       bool x = a.causal && a.seqlen_q > 1;
-      if constexpr (!SMALL) x = x && max(m.key0[0], m.key0[NH - 1]) + 15 > len - a.seqlen_q;
+      if constexpr (!ANY) x = x && max(m.key0[0] + (NH == 1 ? 31 : 15), m.key0[NH - 1] + (NH == 1 ? 31 : 15)) > len - a.seqlen_q;
       return x;
     };
 
@@ -521,7 +562,6 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
       const bool more = k + 1 < mine;
       const Meta m = now;
       const bool whole = m.there == 0xFFFFFFFFu;
-      // Some rows see keys of the chunk that others do not.
       const bool mixed = is_mixed(m);
       if constexpr (C::VLATE) load_v(m);
       // Rows that are no keys as zeros (0 * NaN would be NaN).
@@ -546,8 +586,8 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
       for (int i = 0; i < C::VN; ++i) {
         const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
         if constexpr (C::KV8) {
-          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = codes_to_f16<KV>(u32x2{vd[i][0], vd[i][1]});
-          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col + 8)) = codes_to_f16<KV>(u32x2{vd[i][2], vd[i][3]});
+          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = codes_to_f16<KV, false>(u32x2{vd[i][0], vd[i][1]});
+          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col + 8)) = codes_to_f16<KV, false>(u32x2{vd[i][2], vd[i][3]});
         } else {
           *reinterpret_cast<u32x4*>(tile + swz_off<D>(row, col)) = vd[i];
         }
@@ -566,15 +606,15 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r][h] = f32x4a{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < R; ++r) s[r][h] = f32x4a{zero[r], zero[r], zero[r], zero[r]};
 #pragma unroll
         for (int t = 0; t < C::NSTEP; ++t) {
           s16x8 x;
           if constexpr (C::PAIR) {
             const u32x4 y = __builtin_bit_cast(u32x4, kd[h][t / 2]);
-            x = codes_to_f16<KV>(t % 2 ? u32x2{y[2], y[3]} : u32x2{y[0], y[1]});
+            x = codes_to_f16<KV, true>(t % 2 ? u32x2{y[2], y[3]} : u32x2{y[0], y[1]});
           } else if constexpr (C::KV8) {
-            x = codes_to_f16<KV>(__builtin_bit_cast(u32x2, kd[h][t]));
+            x = codes_to_f16<KV, true>(__builtin_bit_cast(u32x2, kd[h][t]));
           } else {
             x = __builtin_bit_cast(s16x8, kd[h][t]);
           }
@@ -583,37 +623,32 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
         }
       }
       if (more) load_k(now);
-      // Per key: scales (uniform over a half, or the key's own) and position.
-      constexpr int NI = SMALL ? 4 : 1;
+      // Scales and positions: uniform over a page's keys, or each key's own.
+      auto of_key = [&](const auto (&x)[NH], int h, int i) {
+        if constexpr (ANY) return __shfl(x[0], 16 * h + 4 * g4 + i, 64);
+        else return x[NH == 2 ? h : 0];
+      };
+      constexpr int NI = ANY ? 4 : 1;
       float ks[2][NI], wv[2][NI];
-      int pos[2][NI];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (SMALL) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = 16 * h + 4 * g4 + i;
-            ks[h][i] = __shfl(m.ks[0], key, 64);
-            wv[h][i] = __shfl(m.vs[0], key, 64);
-            pos[h][i] = __shfl(m.key0[0], key, 64);
-          }
-        } else {
-          ks[h][0] = m.ks[h];
-          wv[h][0] = m.vs[h];
-          pos[h][0] = m.key0[h] + 4 * g4;
+        for (int i = 0; i < NI; ++i) {
+          ks[h][i] = of_key(m.ks, h, i);
+          wv[h][i] = of_key(m.vs, h, i);
         }
-      }
+      uint32_t scale_top = 0;
       if constexpr (C::KV8) {
-        uint32_t top = __float_as_uint(m.vs[0]) & 0x7FFFFFFFu;
-        if constexpr (SMALL) {
+        scale_top = __float_as_uint(m.vs[0]) & 0x7FFFFFFFu;
+        if constexpr (ANY) {
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+          for (int o = 1; o < 32; o <<= 1) scale_top = max(scale_top, (uint32_t)__shfl_xor((int)scale_top, o, 64));
         } else {
-          top = max(top, __float_as_uint(m.vs[NH - 1]) & 0x7FFFFFFFu);
+          scale_top = max(scale_top, __float_as_uint(m.vs[NH - 1]) & 0x7FFFFFFFu);
         }
-        top = __builtin_amdgcn_readfirstlane(top);
-        if (top > vref) {
-          const uint32_t grown = min((top + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u);
+        scale_top = __builtin_amdgcn_readfirstlane(scale_top);
+        if (scale_top > vref) {
+          const uint32_t grown = min((scale_top + 0x7FFFFFu) & 0x7F800000u, 0x7E800000u);
           const float f = __uint_as_float((uint32_t)max((int)(0x3F800000u + vref - grown), 0));
           vref = grown;
 #pragma unroll
@@ -627,59 +662,86 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
 #pragma unroll
           for (int i = 0; i < NI; ++i) wv[h][i] *= inv;
       }
-      const bool masked = SMALL || !whole || mixed;
+      const bool masked = ANY || !whole || mixed;
       s16x8 p[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        float f[2][NI];  // factor of the logits
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][h][i] *= qscale[r] * ks[h][SMALL ? i : 0];
+          for (int i = 0; i < NI; ++i) f[h][i] = qscale[r] * ks[h][i];
+        uint32_t seen = 0xFFu;  // this lane's keys that its row sees
         if (masked) {
+          seen = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const bool seen = ((m.there >> (16 * h + 4 * g4 + i)) & 1u) && pos[h][SMALL ? i : 0] + (SMALL ? 0 : i) <= klim[r];
-              s[r][h][i] = seen ? s[r][h][i] : kNegInf;
+              const int pos = ANY ? of_key(m.key0, h, i) : m.key0[NH == 2 ? h : 0] + (NH == 2 ? 0 : 16 * h) + 4 * g4 + i;
+              const bool yes = ((m.there >> (16 * h + 4 * g4 + i)) & 1u) && pos <= klim[r];
+              seen |= yes ? 1u << (4 * h + i) : 0u;
             }
         }
+        f32x4a x[2];
         float top = kNegInf;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[r][h][i]);
-        if (__builtin_amdgcn_ballot_w64(top - m_i[r] > 8.f)) {
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float high = fmaxf(m_i[r], top), f = __builtin_amdgcn_exp2f(m_i[r] - high);
-          m_i[r] = high;
-          l_i[r] *= f;
+          for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[r][h][i], f[h][ANY ? i : 0], -m_i[r]);
+        auto hide = [&]() {
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < C::NDB; ++i) acc[r][i] *= f;
+            for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = (seen >> i) & 1u ? x[i / 4][i % 4] : kNegInf;
+          }
+        };
+        hide();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i / 4][i % 4]);
+        if (__builtin_amdgcn_ballot_w64(top > 8.f)) {
+          float high = m_i[r];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              high = fmaxf(high, (seen >> (4 * h + i)) & 1u ? s[r][h][i] * f[h][ANY ? i : 0] : kNegInf);
+          high = fmaxf(high, __shfl_xor(high, 16, 64));
+          high = fmaxf(high, __shfl_xor(high, 32, 64));
+          const float down = __builtin_amdgcn_exp2f(m_i[r] - high);
+          m_i[r] = high;
+          l_i[r] *= down;
+#pragma unroll
+          for (int i = 0; i < C::NDB; ++i) acc[r][i] *= down;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[r][h][i], f[h][ANY ? i : 0], -high);
+          hide();
         }
+        float y[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x = __builtin_amdgcn_exp2f(s[r][h][i] - m_i[r]);
-            l_i[r] += x;
-            float y = C::KV8 ? x * wv[h][SMALL ? i : 0] : x;
-            if (masked) y = s[r][h][i] == kNegInf ? 0.f : y;  // (0 * a scale that is not finite)
-            p[r][4 * h + i] = (short)Elem<CT>::from_f(y);
+            const float e = __builtin_amdgcn_exp2f(x[h][i]);
+            l_i[r] += e;
+            y[4 * h + i] = C::KV8 ? e * wv[h][ANY ? i : 0] : e;
           }
+        if (C::KV8 && __builtin_expect(scale_top >= 0x7F800000u, 0)) {  // (0 * a scale that is not finite)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = x[i / 4][i % 4] == kNegInf ? 0.f : y[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[r][i] = (short)Elem<CT>::from_f(y[i]);
       }
       const int trow = 4 * g4 + (l16 >> 2);
       typedef __attribute__((address_space(3))) s4a lds_s4;
-      auto v_op = [&](int i) -> s16x8 {
+#pragma unroll
+      for (int i = 0; i < C::NDB; ++i) {
         uint16_t* const t = tile + swz_off<D>(trow, 16 * i + 4 * (lane & 3));
         const s4a lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)t);
         const s4a hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(t + 16 * D));
-        return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      };
-#pragma unroll
-      for (int i = 0; i < C::NDB; ++i) {
-        const s16x8 v = v_op(i);
+        const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][i] = mma16x16<CT>(v, p[r], acc[r][i]);
       }
@@ -702,23 +764,24 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, SMALL>::NT)) void paged_att
           int64_t off;
           int pos;
           float vs;
-          if constexpr (SMALL) {
+          if constexpr (ANY) {
             off = far(m.voff[0], key);
             pos = __shfl(m.key0[0], key, 64);
             vs = __shfl(m.vs[0], key, 64);
           } else {
-            off = (key < 16 ? m.voff[0] : m.voff[NH - 1]) + (key & 15) * a.v_stride[1];
-            pos = (key < 16 ? m.key0[0] : m.key0[NH - 1]) + (key & 15);
-            vs = key < 16 ? m.vs[0] : m.vs[NH - 1];
+            const int h = NH == 2 && key >= 16 ? NH - 1 : 0, in = NH == 2 ? key & 15 : key;
+            off = (h ? m.voff[NH - 1] : m.voff[0]) + in * (int64_t)v1;
+            pos = (h ? m.key0[NH - 1] : m.key0[0]) + in;
+            vs = h ? m.vs[NH - 1] : m.vs[0];
           }
 #pragma unroll
           for (int i = 0; i < C::NDB; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const KE c = vbase[off + 16 * i + 4 * g4 + e];
+              const bytes at_v = vbase + off + (16 * i + 4 * g4 + e) * ES;
               float f;
-              if constexpr (C::KV8) f = (c & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
-              else f = Elem<CT>::to_f(c);
+              if constexpr (C::KV8) f = (*at_v & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
+              else f = Elem<CT>::to_f(*reinterpret_cast<const uint16_t*>(at_v));
               if (f - f == 0.f) continue;
 #pragma unroll
               for (int r = 0; r < R; ++r)
