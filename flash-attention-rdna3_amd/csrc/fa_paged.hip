@@ -256,114 +256,154 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
     prev = page;
     prev_at = i;
     if (goes_on) continue;
-    // The segment: rows i .. i + n - 1 but for dropped ones, and its lowest position.
-    int n = P, lowest = P;
+    // The segment: rows i .. i + n - 1 but for dropped ones (the last is not),
+    // and its lowest position.
+    int n = 1, lowest = P;
     for (int j0 = 0; j0 < P; j0 += 64) {
       const int j = j0 + lane;
       const int at = j < P ? page_of[i + j] : -1;
       const uint64_t other = __builtin_amdgcn_ballot_w64(at >= 0 && at != page);
-      if (other) n = min(n, j0 + (int)__builtin_ctzll(other));
-      if (at == page && j < n) lowest = min(lowest, pos_of[i + j]);
+      const uint64_t before = other ? (1ull << __builtin_ctzll(other)) - 1 : ~0ull;  // lanes of the segment
+      const uint64_t own = __builtin_amdgcn_ballot_w64(at == page) & before;
+      if (own) n = j0 + 64 - __builtin_clzll(own);
+      if ((own >> lane) & 1u) lowest = min(lowest, pos_of[i + j]);
       if (other) break;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) lowest = min(lowest, __shfl_xor(lowest, o, 64));
     lowest = __builtin_amdgcn_readfirstlane(lowest);
     const uint16_t* const src = s.src + (t0 - P + i) * s.src_stride[0] + head * s.src_stride[1] + 8 * c;
-    auto mine = [&](int r) { return page_of[i + r] == page; };
-    auto row_of = [&](int r) { return *reinterpret_cast<const s16x8*>(src + r * s.src_stride[0]); };
-
-    if (a.bounds && (item & 1) == 0) {
-      float low[8], high[8];
+    const bool with_bounds = a.bounds && (item & 1) == 0;
+    // Rows r0 + sub, r0 + sub + RPI, ...: N loads in flight, `ok` the rows that are there.
+    auto load = [&](auto count, int r0, s16x8 (&x)[decltype(count)::value]) -> uint32_t {
+      constexpr int N = decltype(count)::value;
+      uint32_t ok = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { low[e] = -kNegInf; high[e] = kNegInf; }
-      uint16_t* const bl = a.bounds + page * a.bounds_stride[0] + head * a.bounds_stride[1] + 8 * c;
-      uint16_t* const bh = bl + a.bounds_stride[2];
-      if (lowest > 0 && sub == 0) {
-        const s16x8 x = *reinterpret_cast<const s16x8*>(bl), y = *reinterpret_cast<const s16x8*>(bh);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { low[e] = EL::to_f((uint16_t)x[e]); high[e] = EL::to_f((uint16_t)y[e]); }
+      for (int u = 0; u < N; ++u) {
+        const int r = r0 + u * RPI + sub;
+        ok |= (r < n && page_of[i + min(r, n - 1)] == page) ? 1u << u : 0u;
+        x[u] = *reinterpret_cast<const s16x8*>(src + min(r, n - 1) * s.src_stride[0]);
       }
-      for (int r = sub; r < n; r += RPI) {
-        if (!mine(r)) continue;
-        const s16x8 x = row_of(r);
+      return ok;
+    };
+    float amax = 0.f, low[8], high[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = EL::to_f((uint16_t)x[e]);
-          low[e] = fminf(low[e], f);   // (a NaN operand leaves the other)
+    for (int e = 0; e < 8; ++e) { low[e] = -kNegInf; high[e] = kNegInf; }
+    auto look = [&](const s16x8& x, bool ok) {
+      if (!ok) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = EL::to_f((uint16_t)x[e]);
+        if constexpr (FMT != FA_KV_SAME) amax = fmaxf(amax, fabsf(f) < __builtin_inff() ? fabsf(f) : 0.f);
+        if (with_bounds) {
+          low[e] = fminf(low[e], f);  // (a NaN operand leaves the other)
           high[e] = fmaxf(high[e], f);
         }
       }
+    };
+    float before = 0.f, after = 1.f;
+    auto settle = [&]() {  // scale, rows of before, bounds
+      if constexpr (FMT != FA_KV_SAME) {
+        using C = Code<FMT>;
 #pragma unroll
-      for (int o = LPR; o < 64; o <<= 1)
+        for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+        after = fmaxf(before, scale_for<FMT>(amax));
+        if (lowest > 0 && after > before) {
+          uint8_t* const dst = reinterpret_cast<uint8_t*>(s.dst) + page * s.dst_stride[0] + head * s.dst_stride[2] + 8 * c;
+          const float ratio = before / after;
+          for (int r = sub; r < lowest; r += RPI) {
+            u32x2* const at = reinterpret_cast<u32x2*>(dst + r * s.dst_stride[1]);
+            const u32x2 w = *at;
+            u32x2 z;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          low[e] = fminf(low[e], __shfl_xor(low[e], o, 64));
-          high[e] = fmaxf(high[e], __shfl_xor(high[e], o, 64));
-        }
-      if (sub == 0) {
-        s16x8 x, y;
+            for (int h = 0; h < 2; ++h) {
+              float x[4];
+              C::unpack(w[h], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { x[e] = (short)EL::from_f(low[e]); y[e] = (short)EL::from_f(high[e]); }
-        *reinterpret_cast<s16x8*>(bl) = x;
-        *reinterpret_cast<s16x8*>(bh) = y;
-      }
-    }
-
-    if constexpr (FMT == FA_KV_SAME) {
-      uint16_t* const dst = reinterpret_cast<uint16_t*>(s.dst) + page * s.dst_stride[0] + head * s.dst_stride[2] + 8 * c;
-      for (int r = sub; r < n; r += RPI)
-        if (mine(r)) *reinterpret_cast<s16x8*>(dst + pos_of[i + r] * s.dst_stride[1]) = row_of(r);
-    } else {
-      using C = Code<FMT>;
-      float amax = 0.f;
-      for (int r = sub; r < n; r += RPI) {
-        if (!mine(r)) continue;
-        const s16x8 x = row_of(r);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float f = fabsf(EL::to_f((uint16_t)x[e]));
-          amax = fmaxf(amax, f < __builtin_inff() ? f : 0.f);
-        }
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-      float* const scale = s.scale + page * s.scale_stride[0] + head * s.scale_stride[1];
-      const float before = lowest > 0 ? *scale : 0.f;
-      const float after = fmaxf(before, scale_for<FMT>(amax));
-      uint8_t* const dst = reinterpret_cast<uint8_t*>(s.dst) + page * s.dst_stride[0] + head * s.dst_stride[2] + 8 * c;
-      if (lowest > 0 && after > before) {
-        const float ratio = before / after;
-        for (int r = sub; r < lowest; r += RPI) {
-          u32x2* const at = reinterpret_cast<u32x2*>(dst + r * s.dst_stride[1]);
-          const u32x2 w = *at;
-          u32x2 z;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[4];
-            C::unpack(w[h], x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= ratio;
-            z[h] = C::pack(x);
+              for (int e = 0; e < 4; ++e) x[e] *= ratio;
+              z[h] = C::pack(x);
+            }
+            *at = z;
           }
-          *at = z;
+        }
+        if (lane == 0) s.scale[page * s.scale_stride[0] + head * s.scale_stride[1]] = after;
+      }
+      if (with_bounds) {
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            low[e] = fminf(low[e], __shfl_xor(low[e], o, 64));
+            high[e] = fmaxf(high[e], __shfl_xor(high[e], o, 64));
+          }
+        if (sub == 0) {
+          uint16_t* const bl = a.bounds + page * a.bounds_stride[0] + head * a.bounds_stride[1] + 8 * c;
+          s16x8 x, y;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { x[e] = (short)EL::from_f(low[e]); y[e] = (short)EL::from_f(high[e]); }
+          *reinterpret_cast<s16x8*>(bl) = x;
+          *reinterpret_cast<s16x8*>(bl + a.bounds_stride[2]) = y;
         }
       }
-      const float inv = 1.f / after;
-      for (int r = sub; r < n; r += RPI) {
-        if (!mine(r)) continue;
-        const s16x8 x = row_of(r);
+    };
+    auto store = [&](const s16x8& x, int r) {
+      const int64_t at = page * s.dst_stride[0] + head * s.dst_stride[2] + pos_of[i + r] * s.dst_stride[1] + 8 * c;
+      if constexpr (FMT == FA_KV_SAME) {
+        *reinterpret_cast<s16x8*>(reinterpret_cast<uint16_t*>(s.dst) + at) = x;
+      } else {
+        const float inv = 1.f / after;
         u32x2 z;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float f[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) f[e] = clamp_code<FMT>(EL::to_f((uint16_t)x[4 * h + e]) * inv);
-          z[h] = C::pack(f);
+          z[h] = Code<FMT>::pack(f);
         }
-        *reinterpret_cast<u32x2*>(dst + pos_of[i + r] * s.dst_stride[1]) = z;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(s.dst) + at) = z;
       }
-      if (lane == 0) *scale = after;
+    };
+    // What was there before, asked for along with the rows.
+    if (lowest > 0) {
+      if constexpr (FMT != FA_KV_SAME) before = s.scale[page * s.scale_stride[0] + head * s.scale_stride[1]];
+      if (with_bounds && sub == 0) {
+        const uint16_t* const bl = a.bounds + page * a.bounds_stride[0] + head * a.bounds_stride[1] + 8 * c;
+        const s16x8 x = *reinterpret_cast<const s16x8*>(bl), y = *reinterpret_cast<const s16x8*>(bl + a.bounds_stride[2]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { low[e] = EL::to_f((uint16_t)x[e]); high[e] = EL::to_f((uint16_t)y[e]); }
+      }
+    }
+    // Up to N loads of rows stay in registers between the two looks at them.
+    auto whole = [&](auto count) {
+      constexpr int N = decltype(count)::value;
+      s16x8 x[N];
+      const uint32_t ok = load(count, 0, x);
+#pragma unroll
+      for (int u = 0; u < N; ++u) look(x[u], (ok >> u) & 1u);
+      settle();
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+        if ((ok >> u) & 1u) store(x[u], u * RPI + sub);
+    };
+    if (n <= RPI) {
+      whole(std::integral_constant<int, 1>{});
+    } else if (n <= 16 * RPI) {
+      whole(std::integral_constant<int, 16>{});
+    } else {
+      using Eight = std::integral_constant<int, 8>;
+      s16x8 x[8];
+      for (int r0 = 0; r0 < n; r0 += 8 * RPI) {
+        const uint32_t ok = load(Eight{}, r0, x);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) look(x[u], (ok >> u) & 1u);
+      }
+      settle();
+      for (int r0 = 0; r0 < n; r0 += 8 * RPI) {
+        const uint32_t ok = load(Eight{}, r0, x);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if ((ok >> u) & 1u) store(x[u], r0 + u * RPI + sub);
+      }
     }
   }
 }
@@ -437,13 +477,13 @@ hipError_t launch_paged_append(const fa_paged_append_params& p, hipStream_t stre
 // depend on the order of a sum; the vector units' rate for 64-bit FMAs hides
 // them behind the bounds' bytes.
 //
-// paged_score_kernel: a lane owns 4 dims of a block (D / 4 lanes a block, 64
-// at D = 512 with 8) and 4 query rows in registers; the 4 rows' sums are
-// folded over the lanes with the rows shared out, so that a step halves what
-// is left to add.  Each block's score goes to the workspace as an integer of
-// the same order.  paged_top_kernel: one workgroup per (sequence, KV head)
-// finds the n_index-th largest by 12-bit digits and writes the chosen ones in
-// index order.
+// paged_score_kernel: a lane owns 8 dims of a block (16 bytes of each bound)
+// and 4 query rows in registers, D / 8 lanes a block; a wave asks for the
+// bounds of several blocks at once.  The 4 rows' sums are folded over the lanes
+// with the rows shared out, so that a step halves what is left to add.  Each
+// block's score goes to the workspace as an integer of the same order.
+// paged_top_kernel: one workgroup per (sequence, KV head) finds the n_index-th
+// largest by 12-bit digits and writes the chosen ones in index order.
 // ---------------------------------------------------------------------------
 namespace {
 constexpr int kScoreThreads = 256;
@@ -474,9 +514,11 @@ __device__ inline int blocks_of(const SelectArgs& a, int b) {
 template <typename Tag, int D>
 __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a) {
   using EL = Elem<Tag>;
-  constexpr int LPB = D / 4 < 64 ? D / 4 : 64;  // lanes of a block
-  constexpr int DPL = D / LPB;                  // dims of a lane: 4, or 8 at D = 512
-  constexpr int BPW = 64 / LPB;                 // blocks a wave reads at a time
+  constexpr int LPB = D / 8;                               // lanes of a block
+  constexpr int BPW = 64 / LPB;                            // blocks a wave reads at a time
+  constexpr int OWN = kScoreBlocks / (kScoreThreads / 64); // blocks of a wave
+  constexpr int PER = OWN / BPW;                           // passes of a wave over them
+  constexpr int AT_ONCE = PER < 4 ? PER : 4;               // passes whose loads are in flight together
   __shared__ uint64_t best[kScoreBlocks];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -487,59 +529,68 @@ __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a
   if (n <= a.p.n_index || first >= n) return;
   const int group = a.p.heads_q / a.p.heads_kv, rows = group * a.p.seqlen_q;
   const int c = lane % LPB, sub = lane / LPB;
-  const uint16_t* const bounds = reinterpret_cast<const uint16_t*>(a.p.key_bounds) + h * a.p.bounds_stride[1] + DPL * c;
-  constexpr int PER = kScoreBlocks / (kScoreThreads / 64) / BPW;  // passes of a wave over its blocks
+  const uint16_t* const bounds = reinterpret_cast<const uint16_t*>(a.p.key_bounds) + h * a.p.bounds_stride[1] + 8 * c;
+  // The pages of the wave's blocks, one a lane (-1: none).
+  int pages = -1;
+  if (lane < OWN && first + wave * OWN + lane < n)
+    pages = a.p.block_table[b * a.p.block_table_stride[0] + (first + wave * OWN + lane) * a.p.block_table_stride[1]];
+  if (pages >= a.p.num_blocks) pages = -1;
+#pragma unroll 1
   for (int r0 = 0; r0 < rows; r0 += kScoreRows) {
-    double pos[kScoreRows][DPL], neg[kScoreRows][DPL];
+    double pos[kScoreRows][8], neg[kScoreRows][8];
 #pragma unroll
     for (int r = 0; r < kScoreRows; ++r) {
       const int row = min(r0 + r, rows - 1);  // (a row twice changes no maximum)
       const int g = row / a.p.seqlen_q, m = row - g * a.p.seqlen_q;
-      const uint16_t* const q = reinterpret_cast<const uint16_t*>(a.p.q) + b * a.p.q_stride[0] +
-                                (h * group + g) * a.p.q_stride[1] + m * a.p.q_stride[2] + DPL * c;
+      const s16x8 q = *reinterpret_cast<const s16x8*>(reinterpret_cast<const uint16_t*>(a.p.q) + b * a.p.q_stride[0] +
+                                                      (h * group + g) * a.p.q_stride[1] + m * a.p.q_stride[2] + 8 * c);
 #pragma unroll
-      for (int e = 0; e < DPL; ++e) {
-        const float x = EL::to_f(q[e]);
+      for (int e = 0; e < 8; ++e) {
+        const float x = EL::to_f((uint16_t)q[e]);
         pos[r][e] = x > 0.f ? (double)x : x == x ? 0.0 : (double)x;  // (NaN in both)
         neg[r][e] = x < 0.f ? (double)x : x == x ? 0.0 : (double)x;
       }
     }
-    for (int i = 0; i < PER; ++i) {
-      const int k = (wave * PER + i) * BPW + sub;  // block of this lane, within the workgroup's
-      const int blk = min(first + k, n - 1);
-      const int page = a.p.block_table[b * a.p.block_table_stride[0] + blk * a.p.block_table_stride[1]];
-      const bool there = page >= 0 && page < a.p.num_blocks;
-      const uint16_t* const lo = bounds + (there ? page : 0) * a.p.bounds_stride[0];
-      const uint16_t* const hi = lo + a.p.bounds_stride[2];
-      double sum[kScoreRows] = {};
+#pragma unroll 1
+    for (int i0 = 0; i0 < PER; i0 += AT_ONCE) {
+      s16x8 lo[AT_ONCE], hi[AT_ONCE];
+      int page[AT_ONCE];
 #pragma unroll
-      for (int e0 = 0; e0 < DPL; e0 += 4) {
-        const s16x4 x = *reinterpret_cast<const s16x4*>(lo + e0), y = *reinterpret_cast<const s16x4*>(hi + e0);
+      for (int u = 0; u < AT_ONCE; ++u) {
+        page[u] = __shfl(pages, (i0 + u) * BPW + sub, 64);
+        const uint16_t* const p = bounds + max(page[u], 0) * a.p.bounds_stride[0];
+        lo[u] = *reinterpret_cast<const s16x8*>(p);
+        hi[u] = *reinterpret_cast<const s16x8*>(p + a.p.bounds_stride[2]);
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double l = EL::to_f((uint16_t)x[e]), u = EL::to_f((uint16_t)y[e]);
+      for (int u = 0; u < AT_ONCE; ++u) {
+        double sum[kScoreRows] = {};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const double l = EL::to_f((uint16_t)lo[u][e]), g = EL::to_f((uint16_t)hi[u][e]);
 #pragma unroll
           for (int r = 0; r < kScoreRows; ++r) {
-            sum[r] = __builtin_fma(pos[r][e0 + e], u, sum[r]);
-            sum[r] = __builtin_fma(neg[r][e0 + e], l, sum[r]);
+            sum[r] = __builtin_fma(pos[r][e], g, sum[r]);
+            sum[r] = __builtin_fma(neg[r][e], l, sum[r]);
           }
         }
-      }
-      // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
-      const bool odd = lane & 1, two = lane & 2;
-      double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
-      u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
-      u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
-      double v = two ? u1 : u0;
-      v += __shfl_xor(two ? u0 : u1, 2, 64);
+        // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
+        const bool odd = lane & 1, two = lane & 2;
+        double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
+        u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
+        u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
+        double v = two ? u1 : u0;
+        v += __shfl_xor(two ? u0 : u1, 2, 64);
 #pragma unroll
-      for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
-      if (v != v) v = __builtin_inf();
-      v = fmax(v, __shfl_xor(v, 1, 64));
-      v = fmax(v, __shfl_xor(v, 2, 64));
-      if (c == 0) {
-        const uint64_t key = there ? order_of(v) : kLowest;
-        best[k] = r0 == 0 ? key : max(best[k], key);
+        for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
+        if (v != v) v = __builtin_inf();
+        v = fmax(v, __shfl_xor(v, 1, 64));
+        v = fmax(v, __shfl_xor(v, 2, 64));
+        if (c == 0) {
+          const int k = wave * OWN + (i0 + u) * BPW + sub;  // block, within the workgroup's
+          const uint64_t key = page[u] >= 0 ? order_of(v) : kLowest;
+          best[k] = r0 == 0 ? key : max(best[k], key);
+        }
       }
     }
   }
@@ -552,14 +603,19 @@ __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a
 }
 
 namespace {
-constexpr int kTopThreads = 256;
+constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64;
 constexpr int kDigit = 12, kBins = 1 << kDigit;
 }  // namespace
 
+// PER: keys a thread holds in registers (index j * kTopThreads + thread), or 0:
+// the keys are read again for every digit.
+template <int PER>
 __global__ __launch_bounds__(kTopThreads) void paged_top_kernel(SelectArgs a) {
   __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t wave_sum[kTopThreads / 64];
+  __shared__ uint32_t wave_sum[kTopWaves];
   __shared__ int32_t found[2];
+  constexpr int TILES = PER ? PER : 1;
+  __shared__ int32_t taken[TILES * kTopWaves], equal[TILES * kTopWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x, b = blockIdx.y;
   const int n = blocks_of(a, b), want = a.p.n_index;
@@ -569,25 +625,48 @@ __global__ __launch_bounds__(kTopThreads) void paged_top_kernel(SelectArgs a) {
     return;
   }
   const uint64_t* const keys = a.keys + ((int64_t)b * a.p.heads_kv + h) * a.p.max_blocks;
+  uint64_t mine[TILES];
+  if constexpr (PER) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = j * kTopThreads + tid;
+      mine[j] = keys[min(i, n - 1)];
+    }
+  }
   // The want-th largest key, digit by digit: `prefix` holds the digits found,
   // `left` how many of the keys that share them are still to be taken.
   uint64_t prefix = 0;
   int left = want;
   for (int top = 64; top > 0; top -= kDigit) {
     const int low = max(top - kDigit, 0), width = top - low;
-    constexpr int PER = kBins / kTopThreads;
+    constexpr int BPT = kBins / kTopThreads;
     for (int i = tid; i < kBins; i += kTopThreads) bins[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kTopThreads) {
-      const uint64_t k = keys[i];
-      if (top == 64 || (k >> top) == (prefix >> top)) atomicAdd(&bins[(k >> low) & ((1u << width) - 1)], 1u);
+    auto count = [&](uint64_t k, bool there) {
+      const bool in = there && (top == 64 || (k >> top) == (prefix >> top));
+      const uint32_t bin = (uint32_t)(k >> low) & ((1u << width) - 1);
+      // Scores share their leading digit: one atomic for the lanes of the
+      // first lane's bin.
+      uint64_t rest = __builtin_amdgcn_ballot_w64(in);
+      if (!rest) return;
+      const uint32_t lead = __shfl(bin, __builtin_ctzll(rest), 64);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == lead);
+      if (lane == __builtin_ctzll(rest)) atomicAdd(&bins[lead], (uint32_t)__builtin_popcountll(same));
+      if (in && bin != lead) atomicAdd(&bins[bin], 1u);
+    };
+    if constexpr (PER) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (j * kTopThreads < n) count(mine[j], j * kTopThreads + tid < n);
+    } else {
+      for (int i0 = 0; i0 < n; i0 += kTopThreads) count(keys[min(i0 + tid, n - 1)], i0 + tid < n);
     }
     __syncthreads();
-    // Thread t sums the bins [t * PER, (t + 1) * PER) from the highest thread down.
-    uint32_t mine = 0;
+    // Thread t sums the bins [t * BPT, (t + 1) * BPT) from the highest thread down.
+    uint32_t sum = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) mine += bins[tid * PER + i];
-    uint32_t above = mine;  // inclusive, over the lanes from this one up
+    for (int i = 0; i < BPT; ++i) sum += bins[tid * BPT + i];
+    uint32_t above = sum;  // inclusive, over the lanes from this one up
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t y = __shfl_down(above, o, 64);
@@ -595,46 +674,70 @@ __global__ __launch_bounds__(kTopThreads) void paged_top_kernel(SelectArgs a) {
     }
     if (lane == 0) wave_sum[wave] = above;
     __syncthreads();
-    above -= mine;
-    for (int w = wave + 1; w < kTopThreads / 64; ++w) above += wave_sum[w];
-    if ((int)above < left && (int)(above + mine) >= left) {
-      int digit = PER - 1;
+    above -= sum;
+    for (int w = wave + 1; w < kTopWaves; ++w) above += wave_sum[w];
+    if ((int)above < left && (int)(above + sum) >= left) {
+      int digit = BPT - 1;
       uint32_t seen = above;
-      while ((int)(seen + bins[tid * PER + digit]) < left) seen += bins[tid * PER + digit--];
-      found[0] = tid * PER + digit;
+      while ((int)(seen + bins[tid * BPT + digit]) < left) seen += bins[tid * BPT + digit--];
+      found[0] = tid * BPT + digit;
       found[1] = left - (int)seen;
+      taken[0] = (int)bins[tid * BPT + digit];
     }
     __syncthreads();
     prefix |= (uint64_t)found[0] << low;
     left = found[1];
+    const bool done = taken[0] == left;  // every key of this digit is in
     __syncthreads();
+    if (done) {
+      left = INT_MAX;  // the keys from `prefix` on are the ones wanted
+      break;
+    }
   }
-  // Keys above `prefix`, and the first `left` equal to it, in index order.
-  int at = 0, equal = 0;
-  for (int i0 = 0; i0 < n; i0 += kTopThreads) {
-    const int i = i0 + tid;
-    const uint64_t k = i < n ? keys[i] : 0;
-    const uint64_t eq = __builtin_amdgcn_ballot_w64(i < n && k == prefix);
-    __syncthreads();
-    if (lane == 0) wave_sum[wave] = __builtin_popcountll(eq);
-    __syncthreads();
-    const uint64_t below = (1ull << lane) - 1;
-    int eq_before = equal + __builtin_popcountll(eq & below);
-    for (int w = 0; w < kTopThreads / 64; ++w) {
-      if (w < wave) eq_before += wave_sum[w];
-      equal += wave_sum[w];
+  // Keys above `prefix`, and the first `left` equal to it, in index order
+  // (left INT_MAX: all that are not below it).
+  const bool all = left == INT_MAX;
+  auto is_eq = [&](uint64_t k) { return !all && k == prefix; };
+  auto is_in = [&](uint64_t k) { return all ? k >= prefix : k > prefix; };
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0, eq_at = 0;
+  for (int i0 = 0; i0 < n; i0 += TILES * kTopThreads) {
+    // Counts of each (tile, wave), then their running sums.
+    if constexpr (!PER) mine[0] = keys[min(i0 + tid, n - 1)];
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+      const bool there = i0 + j * kTopThreads + tid < n;
+      const uint64_t e = __builtin_amdgcn_ballot_w64(there && is_eq(mine[j])), g = __builtin_amdgcn_ballot_w64(there && is_in(mine[j]));
+      if (lane == 0) {
+        equal[j * kTopWaves + wave] = __builtin_popcountll(e);
+        taken[j * kTopWaves + wave] = __builtin_popcountll(g);
+      }
     }
-    const bool take = i < n && (k > prefix || (k == prefix && eq_before < left));
-    const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
     __syncthreads();
-    if (lane == 0) wave_sum[wave] = __builtin_popcountll(tk);
-    __syncthreads();
-    int pos = at + __builtin_popcountll(tk & below);
-    for (int w = 0; w < kTopThreads / 64; ++w) {
-      if (w < wave) pos += wave_sum[w];
-      at += wave_sum[w];
+    static_assert(TILES * kTopWaves <= 64, "one lane for each (tile, wave)");
+    const int my_eq = lane < TILES * kTopWaves ? equal[lane] : 0, my_in = lane < TILES * kTopWaves ? taken[lane] : 0;
+    int eqs = my_eq, ins = my_in;  // inclusive sums over (tile, wave)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(eqs, o, 64), y = __shfl_up(ins, o, 64);
+      if (lane >= o) { eqs += x; ins += y; }
     }
-    if (take) out[pos] = i;
+    const int eq_all = __shfl(eqs, 63, 64), in_all = __shfl(ins, 63, 64);
+    eqs -= my_eq;
+    ins -= my_in;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+      const int i = i0 + j * kTopThreads + tid;
+      const bool there = i < n, e = there && is_eq(mine[j]), g = there && is_in(mine[j]);
+      const uint64_t eb = __builtin_amdgcn_ballot_w64(e), gb = __builtin_amdgcn_ballot_w64(g);
+      const int e_before = eq_at + __shfl(eqs, j * kTopWaves + wave, 64) + __builtin_popcountll(eb & below);
+      const int g_before = at + __shfl(ins, j * kTopWaves + wave, 64) + __builtin_popcountll(gb & below);
+      // Equal keys before this one that are in: the first `left` of them.
+      if (g || (e && e_before < left)) out[g_before + min(e_before, left)] = i;
+    }
+    at += in_all;
+    eq_at += eq_all;
+    __syncthreads();
   }
 }
 
@@ -666,7 +769,10 @@ hipError_t launch_select(const fa_select_params& p, hipStream_t stream) {
     const hipError_t e = p.dtype == FA_DTYPE_F16 ? select_by_dim<f16_t>(a, stream) : select_by_dim<bf16_t>(a, stream);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(paged_top_kernel, dim3(p.heads_kv, p.batch), dim3(kTopThreads), 0, stream, a);
+  const dim3 grid(p.heads_kv, p.batch);
+  if (p.max_blocks <= 4 * kTopThreads) hipLaunchKernelGGL(paged_top_kernel<4>, grid, dim3(kTopThreads), 0, stream, a);
+  else if (p.max_blocks <= 16 * kTopThreads) hipLaunchKernelGGL(paged_top_kernel<16>, grid, dim3(kTopThreads), 0, stream, a);
+  else hipLaunchKernelGGL(paged_top_kernel<0>, grid, dim3(kTopThreads), 0, stream, a);
   return hipGetLastError();
 }
 

@@ -12,6 +12,15 @@ int log2_floor(int n) {
   return s;
 }
 
+// KV heads of a workgroup, as a power of two: as many as fill 256 bytes of a
+// token's row, where they divide the count and leave every head a wave.
+int head_shift(const fa_paged_blocks_params& p, int waves) {
+  int s = 0;
+  const int row = p.head_dim * (p.kv_format == FA_KV_SAME ? 2 : 1);
+  while ((row << s) < 256 && p.heads_kv % (2 << s) == 0 && (2 << s) <= waves) ++s;
+  return s;
+}
+
 PageMode page_mode(const fa_paged_blocks_params& p) {
   const int es = p.kv_format == FA_KV_SAME ? 2 : 1;
   auto small = [](int64_t bytes) { return bytes >= 0 && bytes < (int64_t(1) << 31); };
@@ -24,7 +33,7 @@ PageMode page_mode(const fa_paged_blocks_params& p) {
 struct Plan {
   PageMode pages;
   int r;  // row blocks of 16 that a wave holds: two share the loads and the conversion of a chunk
-  int nrb, rb_rows, shares;
+  int nrb, rb_rows, shares, head_shift;
 };
 
 Plan plan_of(const fa_paged_blocks_params& p) {
@@ -34,7 +43,8 @@ Plan plan_of(const fa_paged_blocks_params& p) {
   w.r = p.kv_format == FA_KV_SAME || p.head_dim > 128 || w.pages == kAnyPages || rows <= 16 ? 1 : 2;
   w.nrb = (int)((rows + 16 * w.r - 1) / (16 * w.r));
   w.rb_rows = (int)std::min<int64_t>(rows, 16 * w.r);
-  const int64_t columns = (int64_t)p.heads_kv * w.nrb;
+  w.head_shift = head_shift(p, 8);  // (rows below 256 bytes: 8 waves)
+  const int64_t columns = (int64_t)(p.heads_kv >> w.head_shift) * w.nrb;
   w.shares = p.shares > 0 ? p.shares
                           : (int)std::max<int64_t>(1, (device_cu_count() + columns - 1) / columns);
   return w;
@@ -50,11 +60,11 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
   auto kern = paged_attn_kernel<Tag, KV, D, R, PAGES>;
   hipError_t e = allow_lds((const void*)kern, C::LDS_BYTES);
   if (e != hipSuccess) return e;
-  const int columns = a.heads_kv * w.nrb;
+  const int columns = (a.heads_kv >> a.head_shift) * w.nrb;
   hipLaunchKernelGGL(kern, dim3((unsigned)(columns * w.shares)), dim3(C::NT), C::LDS_BYTES, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.tickets || w.shares == 1) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, 2 * C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
+  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
@@ -128,6 +138,7 @@ hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
   a.scale_log2 = p.softmax_scale * kLog2e;
   a.causal = p.causal;
   a.shares = w.shares;
+  a.head_shift = w.head_shift;
   a.ws_o = reinterpret_cast<float*>(p.workspace);
   a.ws_ml = a.ws_o + partial_rows(p, w) * p.head_dim;
   // (The merge in the same launch addresses partials by 32-bit offsets.)

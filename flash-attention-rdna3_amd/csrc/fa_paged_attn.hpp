@@ -12,13 +12,16 @@
 //    end of one sequence, whole ones, and the start of another; sequences that
 //    several shares hold are merged from unnormalised partials by the last
 //    workgroup that arrives (or by a second launch).
-//  * Stream.  A wave has one chunk in registers (K in the layout of the matrix
-//    instruction's A operand, V as raw 16-byte pieces that pass through an LDS
-//    tile of the wave and come back transposed) and asks for its next one as
-//    soon as each register is read: V after the tile is written, K after
-//    Q K^T.  Page ids and scales are scalar loads a chunk or two ahead, so that
-//    they do not wait behind the stream.  The step is compiled once: unrolled
-//    over two chunks in flight the code outgrew the instruction cache.
+//  * Stream.  A wave has one chunk in registers, whole rows of K and of V as
+//    16-byte pieces (whole cache lines an instruction; loads in the matrix
+//    instruction's own layout take 64 bytes of a row each and measured 4 %
+//    slower).  It writes them to LDS tiles of its own, asks for its next chunk
+//    at once, and reads K back by rows and V transposed.  Page ids and scales
+//    are scalar loads a chunk or two ahead, so that they do not wait behind
+//    the stream.  A second chunk in registers measured 6 % slower.
+//  * Heads.  A workgroup takes as many KV heads as fill 256 bytes of a token's
+//    row, its waves shared out among them (int8, contexts up to 131072: 179 us
+//    with one head of 128 bytes, 166 with two, 166 with four).
 //  * Types.  8-bit codes are fp16 numbers exactly, so over 8-bit caches the
 //    products run in fp16 whatever the query's type: a bfloat16 query row is
 //    scaled by a power of two to a largest value of 2^14 first (its 8 bits fit;
@@ -62,7 +65,8 @@ struct PagedAttnArgs {
   int32_t batch, heads_q, heads_kv, seqlen_q, bf16;
   float scale_log2;
   int32_t causal;
-  int32_t shares;        // workgroups of a (KV head, row block)
+  int32_t shares;        // workgroups of a (head group, row block)
+  int32_t head_shift;    // log2 of the KV heads of a group: a workgroup's waves share them out
   float* ws_o;           // [2 * shares][heads_kv][row blocks][rows of a block][D]
   float* ws_ml;          // the same without D, pairs (m, l)
   uint32_t* tickets;
@@ -76,21 +80,20 @@ enum PageMode { kOnePage, kTwoPages, kAnyPages };
 template <typename Tag, int KV, int D, int R, int PAGES>
 struct AttnCfg {
   static constexpr bool KV8 = KV != FA_KV_SAME;
-  // Waves: two per SIMD where a chunk and the sums leave room for them.
-  static constexpr int NW = D == 512 || (!KV8 && D == 256) ? 4 : 8;
+  static constexpr int ES = KV8 ? 1 : 2;                      // bytes of an element
+  static constexpr int PPR = D * ES / 16;                     // 16-byte pieces of a row
+  static constexpr int VN = 32 * PPR / 64;                    // loads of 32 rows
+  static constexpr int TILE = 32 * D * ES;                    // bytes of one operand's tile
+  // Waves: two per SIMD where their registers and tiles have room.
+  static constexpr int NW = TILE >= 32768 ? 2 : TILE >= 16384 ? 4 : 8;
   static constexpr int NT = 64 * NW;
   static constexpr int RB = 16 * R;                           // rows of a row block
   static constexpr int NSTEP = D / 32;                        // 32-dim steps of Q K^T
   static constexpr int NDB = D / 16;                          // 16-dim blocks of O
-  static constexpr bool PAIR = KV8 && NSTEP > 1;              // one 16-byte K load for two steps
-  static constexpr int KN = PAIR ? NSTEP / 2 : NSTEP;         // K loads per 16 keys
-  static constexpr int KREGS = KV8 && !PAIR ? 2 : 4;          // registers of one
-  static constexpr int EPP = KV8 ? 16 : 8;                    // elements of a 16-byte V piece
-  static constexpr int PPR = D / EPP;                         // pieces of a row
-  static constexpr int VN = 32 * PPR / 64;                    // V loads per chunk
-  // V of a 16-bit chunk at D = 512 loads at its use: no room for it beside K.
-  static constexpr bool VLATE = !KV8 && D == 512;
-  static constexpr int LOOP_BYTES = NW * 32 * D * 2;          // the V tiles
+  static constexpr bool PAIR = KV8 && NSTEP > 1;              // 16 bytes of K serve two steps
+  // Rows of 128 bytes and more are whole cache lines of one head, read once.
+  static constexpr bool ONCE = D * ES >= 128;
+  static constexpr int LOOP_BYTES = 2 * NW * TILE;
   static constexpr int OLD = D + 4;                           // row stride of the waves' sums (floats)
   static constexpr int MERGE_BYTES = NW * RB * (OLD + 2) * 4;
   static constexpr int LDS_BYTES = (LOOP_BYTES > MERGE_BYTES ? LOOP_BYTES : MERGE_BYTES) + 16;  // + ticket flag
@@ -129,6 +132,13 @@ __device__ inline s16x8 int8x8_to_f16(u32x2 r) {
 template <int KV, bool K> __device__ inline s16x8 codes_to_f16(u32x2 r) {
   if constexpr (KV == FA_KV_INT8) return int8x8_to_f16<K>(r);
   else return fp8x8_to_op<f16_t>(r);
+}
+
+// Byte offset of 16-byte piece c of row r in a tile of rows of N pieces: the
+// pieces of the rows that an access touches together lie in different banks.
+template <int N> __device__ constexpr inline int piece_off(int r, int c) {
+  constexpr int PER = N >= 8 ? 1 : 8 / N;  // rows of 128 bytes
+  return (r * N + (c ^ (r / PER & (N >= 8 ? 7 : N - 1)))) * 16;
 }
 
 constexpr float kFloor = -3.0e38f;  // the running maximum before any key
@@ -233,17 +243,17 @@ __device__ inline int64_t partial_row(const PagedAttnArgs& a, int slot, int hk, 
   return (((int64_t)slot * a.heads_kv + hk) * nrb + rb) * rb_rows;
 }
 
-// Merges the partials of one (sequence, KV head, row block): those of the
+// Merges the partials of one (sequence, head group, row block): those of the
 // workgroups j0 .. j1, the first of them in its second slot.
 template <int D, int NT, bool AGENT>
-__device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hk, int rb, int nrb, int rb_rows, int j0, int j1,
+__device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hg, int rb, int nrb, int rb_rows, int j0, int j1,
                                       int tid) {
-  const int rows = a.heads_q / a.heads_kv * a.seqlen_q;
+  const int rows = a.heads_q / a.heads_kv * a.seqlen_q, heads = 1 << a.head_shift;
   const int here = min(rb_rows, rows - rb * rb_rows);
   const __amdgpu_buffer_rsrc_t ro = rsrc_of(a.ws_o), rm = rsrc_of(a.ws_ml);
   typedef float f32x2a __attribute__((ext_vector_type(2)));
-  for (int i = tid; i < here * (D / 4); i += NT) {
-    const int d = i % (D / 4) * 4, r = i / (D / 4);
+  for (int i = tid; i < heads * here * (D / 4); i += NT) {
+    const int d = i % (D / 4) * 4, r = i / (D / 4) % here, hk = hg * heads + i / (D / 4 * here);
     float M = kFloor, L = 0.f;
     f32x4a o = {0.f, 0.f, 0.f, 0.f};
     for (int j = j0; j <= j1; j += 4) {
@@ -280,16 +290,17 @@ __device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hk, int
 // What the shares' kernels have in common: which share this is, and its place
 // in the line of chunks.
 struct SharePlace {
-  int hk, rb, share, nrb, rb_rows;
-  // KV heads fastest: neighbours in dispatch order read the same pages (with
+  int hg, rb, share, nrb, rb_rows;
+  // Head groups fastest: neighbours in dispatch order read the same pages (with
   // the heads of a key range on one XCD instead: 53 us against 50, 4 x 16384 e4m3).
   __device__ SharePlace(const PagedAttnArgs& a, int rows_of_block) {
     const int rows = a.heads_q / a.heads_kv * a.seqlen_q;
     nrb = (rows + rows_of_block - 1) / rows_of_block;
     rb_rows = min(rows_of_block, rows);
-    hk = blockIdx.x % a.heads_kv;
-    rb = blockIdx.x / a.heads_kv % nrb;
-    share = blockIdx.x / (a.heads_kv * nrb);
+    const int groups = a.heads_kv >> a.head_shift;
+    hg = blockIdx.x % groups;
+    rb = blockIdx.x / groups % nrb;
+    share = blockIdx.x / (groups * nrb);
   }
 };
 
@@ -304,13 +315,13 @@ __device__ inline void arrive(const PagedAttnArgs& a, const SharePlace& w, const
   __syncthreads();
   const int j0 = cut.owner(begin), j1 = cut.owner(begin + all - 1);
   if (tid == 0) {
-    uint32_t* const t = a.tickets + ((int64_t)b * a.heads_kv + w.hk) * w.nrb + w.rb;
+    uint32_t* const t = a.tickets + ((int64_t)b * (a.heads_kv >> a.head_shift) + w.hg) * w.nrb + w.rb;
     const bool last = __hip_atomic_fetch_add(t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(j1 - j0);
     if (last) __hip_atomic_store(t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *flag = last;
   }
   __syncthreads();
-  if (*flag) merge_partials<D, NT, true>(a, b, w.hk, w.rb, w.nrb, w.rb_rows, j0, j1, tid);
+  if (*flag) merge_partials<D, NT, true>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, tid);
 }
 
 // A query row of bfloat16 in a lane's s16x8 pieces -> fp16, scaled by a power
@@ -340,31 +351,33 @@ template <typename Tag, int KV, int D, int R, int PAGES>
 __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_attn_kernel(PagedAttnArgs a) {
   using C = AttnCfg<Tag, KV, D, R, PAGES>;
   using CT = typename std::conditional<C::KV8, f16_t, Tag>::type;  // type of the products
-  using KRaw = typename std::conditional<C::KREGS == 2, u32x2, u32x4>::type;
   constexpr bool ANY = PAGES == kAnyPages;
   constexpr int NH = PAGES == kTwoPages ? 2 : 1;  // pages a chunk is described by
-  constexpr int ES = C::KV8 ? 1 : 2;              // bytes of an element
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g4 = lane >> 4, l16 = lane & 15;
   const int group = a.heads_q / a.heads_kv, rows = group * a.seqlen_q;
   const SharePlace w(a, C::RB);
-  const int hk = w.hk;
+  // The group's heads, each on `streams` waves.
+  const int streams = C::NW >> a.head_shift, hw = wave & ((1 << a.head_shift) - 1), stream = wave >> a.head_shift;
+  const int hk = (w.hg << a.head_shift) + hw;
   const PagedWork work{a, w.rb_rows, w.rb};
-  const Shares cut = work.shares(lane, 2 * C::NW);
+  const Shares cut = work.shares(lane, 2 * streams);
   if (w.share >= cut.count) return;
   const int begin = cut.begin(w.share), end = cut.begin(w.share + 1);
   int b, b_begin;
   work.find(begin, lane, b, b_begin);
 
-  // This lane's K row of a half (l16) and V row of a chunk's first piece.
+  // This lane's piece of a chunk's first rows.
   typedef const unsigned char* bytes;
+  constexpr int RPI = 64 / C::PPR;  // rows of one load
+  const int prow = lane / C::PPR, pcol = lane % C::PPR;
   const bytes kbase = static_cast<bytes>(a.k) + hk * a.k_stride[2], vbase = static_cast<bytes>(a.v) + hk * a.v_stride[2];
-  const bytes klane = kbase + (ANY ? 0 : l16 * a.k_stride[1]) + (C::PAIR || !C::KV8 ? 16 : 8) * g4;
-  constexpr int RPI = 64 / C::PPR;  // V rows of one load
-  const bytes vlane = vbase + (ANY ? 0 : (lane / C::PPR & 15) * a.v_stride[1]) + lane % C::PPR * 16;
-  uint16_t* const tile = reinterpret_cast<uint16_t*>(smem) + wave * (32 * D);
+  const bytes klane = kbase + (ANY ? 0 : (prow & 15) * a.k_stride[1]) + pcol * 16;
+  const bytes vlane = vbase + (ANY ? 0 : (prow & 15) * a.v_stride[1]) + pcol * 16;
+  unsigned char* const ktile = smem + wave * 2 * C::TILE;
+  unsigned char* const vtile = ktile + C::TILE;
   const int mask = (1 << a.shift) - 1;
   typedef const __attribute__((address_space(4))) int32_t const_i32;
   typedef const __attribute__((address_space(4))) float const_f32;
@@ -448,40 +461,38 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
       const uint32_t lo = __shfl((uint32_t)x, from, 64), hi = __shfl((uint32_t)(x >> 32), from, 64);
       return (int64_t)(((uint64_t)hi << 32) | lo);
     };
-    KRaw kd[2][C::KN];
-    u32x4 vd[C::VN];
-    auto load_k = [&](const Meta& m) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        bytes p;
-        if constexpr (ANY) p = klane + far(m.koff[0], 16 * h + l16);
-        else p = klane + (NH == 2 ? m.koff[h] : m.koff[0] + 16 * h * (int64_t)k1);
-#pragma unroll
-        for (int s = 0; s < C::KN; ++s) kd[h][s] = *reinterpret_cast<const KRaw*>(p + (C::PAIR || !C::KV8 ? 64 : 32) * s);
-      }
-    };
-    auto load_v = [&](const Meta& m) {
+    u32x4 kd[C::VN], vd[C::VN];
+    auto load_rows = [&](u32x4 (&to)[C::VN], bytes from, const int64_t (&off)[NH], uint32_t stride) {
 #pragma unroll
       for (int i = 0; i < C::VN; ++i) {
         bytes p;
         if constexpr (ANY) {
-          p = vlane + far(m.voff[0], (64 * i + lane) / C::PPR);
+          p = from + far(off[0], (64 * i + lane) / C::PPR);
         } else if constexpr (RPI > 16) {  // both halves in one load
-          p = vlane + (lane < 32 ? m.voff[0] : NH == 2 ? m.voff[NH - 1] : m.voff[0] + 16 * (int64_t)v1);
+          p = from + (lane < 32 ? off[0] : NH == 2 ? off[NH - 1] : off[0] + 16 * (int64_t)stride);
         } else {
           constexpr int HALF = 16 / (RPI > 16 ? 16 : RPI);  // loads of 16 rows
-          p = vlane + (NH == 2 ? m.voff[i / HALF] + i % HALF * RPI * (int64_t)v1 : m.voff[0] + i * RPI * (int64_t)v1);
+          p = from + (NH == 2 ? off[i / HALF] + i % HALF * RPI * (int64_t)stride : off[0] + i * RPI * (int64_t)stride);
         }
-        vd[i] = *reinterpret_cast<const u32x4*>(p);
+        // (Nontemporal where a line is one head's alone: int8, D = 128, 166 ->
+        // 154 us; D = 64, whose lines two waves read, 200 -> 217.)
+        if constexpr (C::ONCE) to[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+        else to[i] = *reinterpret_cast<const u32x4*>(p);
       }
     };
-    const int mine = cnt > wave ? (cnt - wave + C::NW - 1) / C::NW : 0;
-    auto chunk = [&](int k) { return min(c0 + wave + C::NW * k, c0 + cnt - 1); };
-    Ahead next, later;  // of the chunks k + 1 and k + 2
+    auto load = [&](const Meta& m) {
+      load_rows(kd, klane, m.koff, k1);
+      load_rows(vd, vlane, m.voff, v1);
+    };
+    const int mine = cnt > stream ? (cnt - stream + streams - 1) / streams : 0;
+    auto chunk = [&](int k) { return min(c0 + stream + streams * k, c0 + cnt - 1); };
+    Ahead first, next;  // of the chunk in flight and the one behind it
+    int later[NH];      // logical blocks of the one after that
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      next.logical[h] = logical_of(first_key(chunk(0), h));
-      later.logical[h] = logical_of(first_key(chunk(1), h));
+      first.logical[h] = logical_of(first_key(chunk(0), h));
+      next.logical[h] = logical_of(first_key(chunk(1), h));
+      later[h] = logical_of(first_key(chunk(2), h));
     }
 
     // --- Q -----------------------------------------------------------------
@@ -505,15 +516,11 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     }
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
+      first.page[h] = page_of(first.logical[h]);
       next.page[h] = page_of(next.logical[h]);
-      later.page[h] = page_of(later.logical[h]);
     }
-    Meta now = describe(chunk(0), next);
-    load_v(now);
-    load_k(now);
-    next = later;
-#pragma unroll
-    for (int h = 0; h < NH; ++h) later.logical[h] = logical_of(first_key(chunk(2), h));
+    Meta ahead = describe(chunk(0), first);
+    load(ahead);
     float zero[R];  // first value of Q K^T's sums
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -559,11 +566,9 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
 
 #pragma unroll 1
     for (int k = 0; k < mine; ++k) {
-      const bool more = k + 1 < mine;
-      const Meta m = now;
+      const Meta m = ahead;
       const bool whole = m.there == 0xFFFFFFFFu;
       const bool mixed = is_mixed(m);
-      if constexpr (C::VLATE) load_v(m);
       // Rows that are no keys as zeros (0 * NaN would be NaN).
       if (!whole) {
 #pragma unroll
@@ -584,45 +589,51 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
       }
 #pragma unroll
       for (int i = 0; i < C::VN; ++i) {
-        const int piece = 64 * i + lane, row = piece / C::PPR, col = piece % C::PPR * C::EPP;
-        if constexpr (C::KV8) {
-          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col)) = codes_to_f16<KV, false>(u32x2{vd[i][0], vd[i][1]});
-          *reinterpret_cast<s16x8*>(tile + swz_off<D>(row, col + 8)) = codes_to_f16<KV, false>(u32x2{vd[i][2], vd[i][3]});
-        } else {
-          *reinterpret_cast<u32x4*>(tile + swz_off<D>(row, col)) = vd[i];
-        }
+        const int row = (64 * i + lane) / C::PPR;
+        *reinterpret_cast<u32x4*>(ktile + piece_off<C::PPR>(row, pcol)) = kd[i];
+        if constexpr (C::KV8) *reinterpret_cast<u32x4*>(vtile + piece_off<C::PPR>(row, pcol)) = vd[i];
+        else *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(vtile) + swz_off<D>(row, 8 * pcol)) = vd[i];
       }
-      if (more) {
-        now = describe(chunk(k + 1), next);
-        if constexpr (!C::VLATE) load_v(now);
+      if (k + 1 < mine) {
+        ahead = describe(chunk(k + 1), next);
+        load(ahead);
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
-          next.logical[h] = later.logical[h];
-          next.page[h] = page_of(later.logical[h]);
-          later.logical[h] = logical_of(first_key(chunk(k + 3), h));
+          next.logical[h] = later[h];
+          next.page[h] = page_of(later[h]);
+          later[h] = logical_of(first_key(chunk(k + 3), h));
         }
       }
       f32x4a s[R][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const int row = 16 * h + l16;
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r][h] = f32x4a{zero[r], zero[r], zero[r], zero[r]};
+        if constexpr (C::PAIR) {
 #pragma unroll
-        for (int t = 0; t < C::NSTEP; ++t) {
-          s16x8 x;
-          if constexpr (C::PAIR) {
-            const u32x4 y = __builtin_bit_cast(u32x4, kd[h][t / 2]);
-            x = codes_to_f16<KV, true>(t % 2 ? u32x2{y[2], y[3]} : u32x2{y[0], y[1]});
-          } else if constexpr (C::KV8) {
-            x = codes_to_f16<KV, true>(__builtin_bit_cast(u32x2, kd[h][t]));
-          } else {
-            x = __builtin_bit_cast(s16x8, kd[h][t]);
+          for (int t = 0; t < C::NSTEP; t += 2) {
+            const u32x4 y = *reinterpret_cast<const u32x4*>(ktile + piece_off<C::PPR>(row, 2 * t + g4));
+            const s16x8 lo = codes_to_f16<KV, true>(u32x2{y[0], y[1]}), hi = codes_to_f16<KV, true>(u32x2{y[2], y[3]});
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              s[r][h] = mma16x16<CT>(lo, q[r][t], s[r][h]);
+              s[r][h] = mma16x16<CT>(hi, q[r][t + 1], s[r][h]);
+            }
           }
+        } else {
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r][h] = mma16x16<CT>(x, q[r][t], s[r][h]);
+          for (int t = 0; t < C::NSTEP; ++t) {
+            s16x8 x;
+            if constexpr (C::KV8)
+              x = codes_to_f16<KV, true>(*reinterpret_cast<const u32x2*>(ktile + piece_off<C::PPR>(row, g4 / 2) + g4 % 2 * 8));
+            else
+              x = *reinterpret_cast<const s16x8*>(ktile + piece_off<C::PPR>(row, 4 * t + g4));
+#pragma unroll
+            for (int r = 0; r < R; ++r) s[r][h] = mma16x16<CT>(x, q[r][t], s[r][h]);
+          }
         }
       }
-      if (more) load_k(now);
       // Scales and positions: uniform over a page's keys, or each key's own.
       auto of_key = [&](const auto (&x)[NH], int h, int i) {
         if constexpr (ANY) return __shfl(x[0], 16 * h + 4 * g4 + i, 64);
@@ -734,14 +745,26 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[r][i] = (short)Elem<CT>::from_f(y[i]);
       }
-      const int trow = 4 * g4 + (l16 >> 2);
-      typedef __attribute__((address_space(3))) s4a lds_s4;
+      // V^T: group g4's slots are the keys 4 g4 + 0 .. 3 and 16 + 4 g4 + 0 .. 3, as
+      // in the scores.
 #pragma unroll
       for (int i = 0; i < C::NDB; ++i) {
-        uint16_t* const t = tile + swz_off<D>(trow, 16 * i + 4 * (lane & 3));
-        const s4a lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)t);
-        const s4a hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(t + 16 * D));
-        const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        s16x8 v;
+        if constexpr (C::KV8) {
+          // Lanes 2 j and 2 j + 1 of a group of 16 name the two halves of slot j's
+          // row; lane l gets column l of the eight.
+          typedef int i32x2a __attribute__((ext_vector_type(2)));
+          typedef __attribute__((address_space(3))) i32x2a lds_i2;
+          const int row = (l16 >> 3) * 16 + 4 * g4 + (l16 >> 1 & 3);
+          unsigned char* const t = vtile + piece_off<C::PPR>(row, i) + 8 * (l16 & 1);
+          v = codes_to_f16<KV, false>(__builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)t)));
+        } else {
+          typedef __attribute__((address_space(3))) s4a lds_s4;
+          uint16_t* const t = reinterpret_cast<uint16_t*>(vtile) + swz_off<D>(4 * g4 + (l16 >> 2), 16 * i + 4 * (lane & 3));
+          const s4a lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)t);
+          const s4a hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(t + 16 * D));
+          v = s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][i] = mma16x16<CT>(v, p[r], acc[r][i]);
       }
@@ -778,7 +801,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
           for (int i = 0; i < C::NDB; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const bytes at_v = vbase + off + (16 * i + 4 * g4 + e) * ES;
+              const bytes at_v = vbase + off + (16 * i + 4 * g4 + e) * C::ES;
               float f;
               if constexpr (C::KV8) f = (*at_v & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
               else f = Elem<CT>::to_f(*reinterpret_cast<const uint16_t*>(at_v));
@@ -801,7 +824,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     for (int r = 0; r < R; ++r) {
       l_i[r] += __shfl_xor(l_i[r], 16, 64);
       l_i[r] += __shfl_xor(l_i[r], 32, 64);
-      const int row = wave * C::RB + 16 * r + l16;
+      const int row = wave * C::RB + 16 * r + l16;  // (waves of a head: hw, hw + heads, ...)
       if (16 * r + l16 < w.rb_rows) {
         float* const st = so + row * C::OLD + 4 * g4;
 #pragma unroll
@@ -815,31 +838,33 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     __syncthreads();
     const bool complete = cnt == all;
     const int here = min(w.rb_rows, rows - w.rb * C::RB);
-    const int64_t part = partial_row(a, 2 * w.share + (c0 == 0 ? 1 : 0), hk, w.rb, w.nrb, w.rb_rows);
-    for (int i = tid; i < here * (D / 4); i += C::NT) {
-      const int d = i % (D / 4) * 4, r = i / (D / 4);
-      float M = sm[r];
-#pragma unroll
-      for (int v = 1; v < C::NW; ++v) M = fmaxf(M, sm[v * C::RB + r]);
+    const int heads = 1 << a.head_shift;
+    for (int i = tid; i < heads * here * (D / 4); i += C::NT) {
+      const int d = i % (D / 4) * 4, r = i / (D / 4) % here, h = i / (D / 4 * here);
+      float M = kFloor;
+      for (int v = h; v < C::NW; v += heads) M = fmaxf(M, sm[v * C::RB + r]);
       float L = 0.f;
       f32x4a o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int v = 0; v < C::NW; ++v) {
+      for (int v = h; v < C::NW; v += heads) {
         const float f = __builtin_amdgcn_exp2f(sm[v * C::RB + r] - M);
         L += sl[v * C::RB + r] * f;
         o += *reinterpret_cast<const f32x4a*>(so + (v * C::RB + r) * C::OLD + d) * f;
       }
+      const int head = (w.hg << a.head_shift) + h;
       if (complete) {
-        store_out(a, b, hk, w.rb * C::RB + r, d, o * (L == 0.f ? 0.f : 1.f / L));
-      } else if (a.tickets) {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rsrc_of(a.ws_o), (int)(((part + r) * D + d) * 4), 0, kAgent);
+        store_out(a, b, head, w.rb * C::RB + r, d, o * (L == 0.f ? 0.f : 1.f / L));
+        continue;
+      }
+      const int64_t part = partial_row(a, 2 * w.share + (c0 == 0 ? 1 : 0), head, w.rb, w.nrb, w.rb_rows) + r;
+      if (a.tickets) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rsrc_of(a.ws_o), (int)((part * D + d) * 4), 0, kAgent);
         if (d == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, rsrc_of(a.ws_ml), (int)((part + r) * 8), 0, kAgent);
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(M), __float_as_uint(L)}, rsrc_of(a.ws_ml), (int)(part * 8), 0, kAgent);
       } else {
-        *reinterpret_cast<f32x4a*>(a.ws_o + (part + r) * D + d) = o;
+        *reinterpret_cast<f32x4a*>(a.ws_o + part * D + d) = o;
         if (d == 0) {
-          a.ws_ml[2 * (part + r)] = M;
-          a.ws_ml[2 * (part + r) + 1] = L;
+          a.ws_ml[2 * part] = M;
+          a.ws_ml[2 * part + 1] = L;
         }
       }
     }
@@ -853,19 +878,19 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
 }
 
 // The merge as a launch of its own: grid (KV heads * row blocks, batch).
-// LEAST: the fewest chunks of a share, as in the kernel that wrote the partials.
-template <int D, int RB, int LEAST>
+// NW: the waves of the kernel that wrote the partials.
+template <int D, int RB, int NW>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, b = blockIdx.y;
   const SharePlace w(a, RB);
   const PagedWork work{a, w.rb_rows, w.rb};
-  const Shares cut = work.shares(lane, LEAST);
+  const Shares cut = work.shares(lane, 2 * (NW >> a.head_shift));
   int begin = 0;
   for (int b0 = 0; b0 < b; b0 += 64) begin += b0 + lane < b ? work.chunks(b0 + lane) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) begin += __shfl_xor(begin, o, 64);
   const int j0 = cut.owner(begin), j1 = cut.owner(begin + work.chunks(b) - 1);
-  if (j0 != j1) merge_partials<D, 256, false>(a, b, w.hk, w.rb, w.nrb, w.rb_rows, j0, j1, threadIdx.x);
+  if (j0 != j1) merge_partials<D, 256, false>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, threadIdx.x);
 }
 
 }  // namespace fa
