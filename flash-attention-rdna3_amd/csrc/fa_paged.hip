@@ -167,7 +167,12 @@ template <> struct Code<FA_KV_E4M3> {
   static constexpr float kTop = 448.f;
   static constexpr int kTopExp = 8;
   static constexpr uint32_t kTopMant = 0x600000u;
-  // Four codes of |x| <= 448 or NaN.
+  // Four codes of x * inv, |x * inv| <= top.
+  __device__ static uint32_t pack_finite(const float* x, float inv) {
+    const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+    return pack(y);
+  }
+  // Four codes of |x| <= top or NaN.
   __device__ static uint32_t pack(const float* x) {
     const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
@@ -183,6 +188,14 @@ template <> struct Code<FA_KV_INT8> {
   static constexpr float kTop = 127.f;
   static constexpr int kTopExp = 6;
   static constexpr uint32_t kTopMant = 0x7E0000u;
+  // Added to 1.5 * 2^23 a value is rounded to a whole number in the low bits.
+  __device__ static uint32_t pack_finite(const float* x, float inv) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(__builtin_fmaf(x[i], inv, 12582912.f));
+    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000C0Cu);
+    return lo | hi;
+  }
   __device__ static uint32_t pack(const float* x) {
     uint32_t w = 0;
 #pragma unroll
@@ -218,7 +231,9 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int P = 1 << a.shift;
-  const int64_t t0 = (int64_t)blockIdx.x * a.chunk;
+  // Neighbouring workgroups take the heads of the same tokens, K's, then V's.
+  const int groups = (2 * a.heads_kv + kAppendWaves - 1) / kAppendWaves;
+  const int64_t t0 = (int64_t)(blockIdx.x / groups) * a.chunk;
   // Token t0 - P + i at entry i: the chunk, and P rows before and behind it.
   const int span = a.chunk + 2 * P;
   int32_t* const page_of = staged;
@@ -237,25 +252,36 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
     pos_of[i] = pos;
   }
   __syncthreads();
-  const int item = blockIdx.y * kAppendWaves + wave;
+  const int item = blockIdx.x % groups * kAppendWaves + wave;
   if (item >= 2 * a.heads_kv) return;
-  const int head = item >> 1;
-  const AppendSide& s = a.side[item & 1];
+  const bool is_key = item < a.heads_kv;
+  const int head = is_key ? item : item - a.heads_kv;
+  const AppendSide& s = a.side[is_key ? 0 : 1];
   const int c = lane % LPR, sub = lane / LPR;
-  // Page of the last row that is not dropped, within the P rows before.
+  // Page and entry of the last row that is not dropped, within the P rows before.
   int prev = -1, prev_at = -1;
   for (int i0 = 0; i0 < P; i0 += 64) {
-    const uint64_t kept = __builtin_amdgcn_ballot_w64(i0 + lane < P && page_of[i0 + lane] >= 0);
-    if (kept) prev_at = i0 + 63 - __builtin_clzll(kept);
+    const int at = i0 + lane < P ? page_of[i0 + lane] : -1;
+    const uint64_t kept = __builtin_amdgcn_ballot_w64(at >= 0);
+    if (kept) {
+      prev_at = i0 + 63 - __builtin_clzll(kept);
+      prev = __builtin_amdgcn_readlane(at, 63 - __builtin_clzll(kept));
+    }
   }
-  if (prev_at >= 0) prev = __builtin_amdgcn_readfirstlane(page_of[prev_at]);
-  for (int i = P; i < P + a.chunk; ++i) {
+  // The first rows of segments among the chunk's (at most 64): those that no
+  // row of the same page precedes within P rows, dropped ones left out.
+  uint64_t leaders;
+  {
+    const int at = lane < a.chunk ? page_of[P + lane] : -1;
+    const uint64_t kept = __builtin_amdgcn_ballot_w64(at >= 0), under = kept & ((1ull << lane) - 1);
+    const int from = under ? 63 - __builtin_clzll(under) : 0;
+    const int there = __shfl(at, from, 64);  // (every lane takes part)
+    const int page_before = under ? there : prev, entry_before = under ? P + from : prev_at;
+    leaders = __builtin_amdgcn_ballot_w64(at >= 0 && !(at == page_before && P + lane - entry_before < P));
+  }
+  for (; leaders; leaders &= leaders - 1) {
+    const int i = P + (int)__builtin_ctzll(leaders);
     const int page = __builtin_amdgcn_readfirstlane(page_of[i]);
-    if (page < 0) continue;
-    const bool goes_on = page == prev && i - prev_at < P;
-    prev = page;
-    prev_at = i;
-    if (goes_on) continue;
     // The segment: rows i .. i + n - 1 but for dropped ones (the last is not),
     // and its lowest position.
     int n = 1, lowest = P;
@@ -273,7 +299,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
     for (int o = 32; o > 0; o >>= 1) lowest = min(lowest, __shfl_xor(lowest, o, 64));
     lowest = __builtin_amdgcn_readfirstlane(lowest);
     const uint16_t* const src = s.src + (t0 - P + i) * s.src_stride[0] + head * s.src_stride[1] + 8 * c;
-    const bool with_bounds = a.bounds && (item & 1) == 0;
+    const bool with_bounds = a.bounds && is_key;
     // Rows r0 + sub, r0 + sub + RPI, ...: N loads in flight, `ok` the rows that are there.
     auto load = [&](auto count, int r0, s16x8 (&x)[decltype(count)::value]) -> uint32_t {
       constexpr int N = decltype(count)::value;
@@ -286,20 +312,47 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
       }
       return ok;
     };
+    // |x| of 16-bit values order as whole numbers do: two maxima at a time.
+    // Infinities and NaN, which have no part in the scale, are the largest: a
+    // segment that has some is looked at again without them.
+    constexpr uint32_t kExp = std::is_same<Tag, bf16_t>::value ? 0x7F80u : 0x7C00u;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
     float amax = 0.f, low[8], high[8];
+    bool finite = true;
 #pragma unroll
     for (int e = 0; e < 8; ++e) { low[e] = -kNegInf; high[e] = kNegInf; }
     auto look = [&](const s16x8& x, bool ok) {
       if (!ok) return;
+      if constexpr (FMT != FA_KV_SAME) {
+        const u32x4 y = __builtin_bit_cast(u32x4, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = EL::to_f((uint16_t)x[e]);
-        if constexpr (FMT != FA_KV_SAME) amax = fmaxf(amax, fabsf(f) < __builtin_inff() ? fabsf(f) : 0.f);
-        if (with_bounds) {
+        for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, y[e] & 0x7FFF7FFFu));
+      }
+      if (with_bounds) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = EL::to_f((uint16_t)x[e]);
           low[e] = fminf(low[e], f);  // (a NaN operand leaves the other)
           high[e] = fmaxf(high[e], f);
         }
       }
+    };
+    auto look_again = [&](const s16x8& x, bool ok) {
+      if (!ok) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = fabsf(EL::to_f((uint16_t)x[e]));
+        amax = fmaxf(amax, f < __builtin_inff() ? f : 0.f);
+      }
+    };
+    // After the first look: the largest value, and whether all are finite.
+    auto all_finite = [&]() -> bool {
+      if constexpr (FMT == FA_KV_SAME) return true;
+      const uint16_t t = top[0] > top[1] ? top[0] : top[1];
+      finite = __builtin_amdgcn_ballot_w64(t >= kExp) == 0;
+      if (finite) amax = EL::to_f(t);
+      return finite;
     };
     float before = 0.f, after = 1.f;
     auto settle = [&]() {  // scale, rows of before, bounds
@@ -357,8 +410,14 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
         for (int h = 0; h < 2; ++h) {
           float f[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) f[e] = clamp_code<FMT>(EL::to_f((uint16_t)x[4 * h + e]) * inv);
-          z[h] = Code<FMT>::pack(f);
+          for (int e = 0; e < 4; ++e) f[e] = EL::to_f((uint16_t)x[4 * h + e]);
+          if (finite) {
+            z[h] = Code<FMT>::pack_finite(f, inv);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = clamp_code<FMT>(f[e] * inv);
+            z[h] = Code<FMT>::pack(f);
+          }
         }
         *reinterpret_cast<u32x2*>(reinterpret_cast<uint8_t*>(s.dst) + at) = z;
       }
@@ -380,7 +439,15 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
       const uint32_t ok = load(count, 0, x);
 #pragma unroll
       for (int u = 0; u < N; ++u) look(x[u], (ok >> u) & 1u);
+      if (!all_finite()) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) look_again(x[u], (ok >> u) & 1u);
+      }
       settle();
+      // (The rows as new values: the compiler would otherwise keep their 32-bit
+      // forms from one look to the other, 230 registers in all.)
+#pragma unroll
+      for (int u = 0; u < N; ++u) asm("" : "+v"(x[u]));
 #pragma unroll
       for (int u = 0; u < N; ++u)
         if ((ok >> u) & 1u) store(x[u], u * RPI + sub);
@@ -397,6 +464,13 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
 #pragma unroll
         for (int u = 0; u < 8; ++u) look(x[u], (ok >> u) & 1u);
       }
+      if (!all_finite()) {
+        for (int r0 = 0; r0 < n; r0 += 8 * RPI) {
+          const uint32_t ok = load(Eight{}, r0, x);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) look_again(x[u], (ok >> u) & 1u);
+        }
+      }
       settle();
       for (int r0 = 0; r0 < n; r0 += 8 * RPI) {
         const uint32_t ok = load(Eight{}, r0, x);
@@ -410,8 +484,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void paged_append_kernel(AppendA
 
 template <typename Tag, int FMT, int D>
 static hipError_t run_append(const AppendArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.num_tokens + a.chunk - 1) / a.chunk), (2 * a.heads_kv + kAppendWaves - 1) / kAppendWaves);
-  hipLaunchKernelGGL((paged_append_kernel<Tag, FMT, D>), grid, dim3(64 * kAppendWaves),
+  const int64_t groups = (2 * a.heads_kv + kAppendWaves - 1) / kAppendWaves;
+  const int64_t grid = groups * (((int64_t)a.num_tokens + a.chunk - 1) / a.chunk);
+  if (grid > INT_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((paged_append_kernel<Tag, FMT, D>), dim3((unsigned)grid), dim3(64 * kAppendWaves),
                      2 * (a.chunk + (2 << a.shift)) * sizeof(int32_t), stream, a);
   return hipGetLastError();
 }
@@ -487,7 +563,7 @@ hipError_t launch_paged_append(const fa_paged_append_params& p, hipStream_t stre
 // ---------------------------------------------------------------------------
 namespace {
 constexpr int kScoreThreads = 256;
-constexpr int kScoreBlocks = 64;  // blocks of a workgroup
+constexpr int kScoreMost = 512;   // most blocks of a workgroup
 constexpr int kScoreRows = 4;     // query rows at a time
 constexpr uint64_t kAlways = ~0ull;
 constexpr uint64_t kLowest = 0x000FFFFFFFFFFFFFull;  // order_of(-infinity)
@@ -496,6 +572,7 @@ struct SelectArgs {
   fa_select_params p;
   uint64_t* keys;  // (batch, heads_kv, max_blocks)
   int32_t shift;
+  int32_t span;    // blocks of a scoring workgroup: 64 for each round of its waves' 16
 };
 
 // An integer that orders as the double does (NaN: as +infinity; -0 as 0).
@@ -514,27 +591,32 @@ __device__ inline int blocks_of(const SelectArgs& a, int b) {
 template <typename Tag, int D>
 __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a) {
   using EL = Elem<Tag>;
-  constexpr int LPB = D / 8;                               // lanes of a block
-  constexpr int BPW = 64 / LPB;                            // blocks a wave reads at a time
-  constexpr int OWN = kScoreBlocks / (kScoreThreads / 64); // blocks of a wave
-  constexpr int PER = OWN / BPW;                           // passes of a wave over them
-  constexpr int AT_ONCE = PER < 4 ? PER : 4;               // passes whose loads are in flight together
-  __shared__ uint64_t best[kScoreBlocks];
+  constexpr int LPB = D / 8;                       // lanes of a block
+  constexpr int BPW = 64 / LPB;                    // blocks a wave reads at a time
+  constexpr int WAVES = kScoreThreads / 64;
+  constexpr int OWN = 16;                          // blocks of a wave in a round
+  constexpr int PER = OWN / BPW;                   // reads for them
+  constexpr int AT_ONCE = PER < 4 ? PER : 4;       // reads in flight together, and as many behind them
+  __shared__ uint64_t best[kScoreMost];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.y, b = blockIdx.z;
   const int n = blocks_of(a, b);
-  const int first = blockIdx.x * kScoreBlocks;
+  const int first = blockIdx.x * a.span, here = min(a.span, n - first);
   // A choice is only made among more than n_index blocks.
-  if (n <= a.p.n_index || first >= n) return;
+  if (n <= a.p.n_index || here <= 0) return;
   const int group = a.p.heads_q / a.p.heads_kv, rows = group * a.p.seqlen_q;
   const int c = lane % LPB, sub = lane / LPB;
   const uint16_t* const bounds = reinterpret_cast<const uint16_t*>(a.p.key_bounds) + h * a.p.bounds_stride[1] + 8 * c;
-  // The pages of the wave's blocks, one a lane (-1: none).
-  int pages = -1;
-  if (lane < OWN && first + wave * OWN + lane < n)
-    pages = a.p.block_table[b * a.p.block_table_stride[0] + (first + wave * OWN + lane) * a.p.block_table_stride[1]];
-  if (pages >= a.p.num_blocks) pages = -1;
+  const int32_t* const table = a.p.block_table + b * a.p.block_table_stride[0];
+  // Blocks of the workgroup: round j of wave w holds j * 64 + 16 w + 0 .. 15.
+  const int rounds = (here + OWN * WAVES - 1) / (OWN * WAVES);
+  auto pages_of = [&](int j) {  // one a lane, -1: none
+    const int k = j * OWN * WAVES + wave * OWN + lane % OWN;
+    int page = -1;
+    if (j < rounds && k < here) page = table[(int64_t)(first + k) * a.p.block_table_stride[1]];
+    return page < a.p.num_blocks ? page : -1;
+  };
 #pragma unroll 1
   for (int r0 = 0; r0 < rows; r0 += kScoreRows) {
     double pos[kScoreRows][8], neg[kScoreRows][8];
@@ -551,59 +633,76 @@ __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a
         neg[r][e] = x < 0.f ? (double)x : x == x ? 0.0 : (double)x;
       }
     }
-#pragma unroll 1
-    for (int i0 = 0; i0 < PER; i0 += AT_ONCE) {
-      s16x8 lo[AT_ONCE], hi[AT_ONCE];
-      int page[AT_ONCE];
+    int pages = pages_of(0), pages_next = pages_of(1);
+    s16x8 lo[AT_ONCE], hi[AT_ONCE];
+    int page[AT_ONCE];
+    auto ask = [&](int from, int i0) {
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        page[u] = __shfl(pages, (i0 + u) * BPW + sub, 64);
+        page[u] = __shfl(from, (i0 + u) * BPW + sub, 64);
         const uint16_t* const p = bounds + max(page[u], 0) * a.p.bounds_stride[0];
         lo[u] = *reinterpret_cast<const s16x8*>(p);
         hi[u] = *reinterpret_cast<const s16x8*>(p + a.p.bounds_stride[2]);
       }
+    };
+    ask(pages, 0);
+#pragma unroll 1
+    for (int j = 0; j < rounds; ++j) {
+#pragma unroll 1
+      for (int i0 = 0; i0 < PER; i0 += AT_ONCE) {
+        s16x8 l_now[AT_ONCE], h_now[AT_ONCE];
+        int p_now[AT_ONCE];
 #pragma unroll
-      for (int u = 0; u < AT_ONCE; ++u) {
-        double sum[kScoreRows] = {};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double l = EL::to_f((uint16_t)lo[u][e]), g = EL::to_f((uint16_t)hi[u][e]);
-#pragma unroll
-          for (int r = 0; r < kScoreRows; ++r) {
-            sum[r] = __builtin_fma(pos[r][e], g, sum[r]);
-            sum[r] = __builtin_fma(neg[r][e], l, sum[r]);
-          }
+        for (int u = 0; u < AT_ONCE; ++u) { l_now[u] = lo[u]; h_now[u] = hi[u]; p_now[u] = page[u]; }
+        const bool turn = i0 + AT_ONCE >= PER;
+        if (turn) {
+          pages = pages_next;
+          pages_next = pages_of(j + 2);
         }
-        // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
-        const bool odd = lane & 1, two = lane & 2;
-        double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
-        u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
-        u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
-        double v = two ? u1 : u0;
-        v += __shfl_xor(two ? u0 : u1, 2, 64);
+        ask(pages, turn ? 0 : i0 + AT_ONCE);
 #pragma unroll
-        for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
-        if (v != v) v = __builtin_inf();
-        v = fmax(v, __shfl_xor(v, 1, 64));
-        v = fmax(v, __shfl_xor(v, 2, 64));
-        if (c == 0) {
-          const int k = wave * OWN + (i0 + u) * BPW + sub;  // block, within the workgroup's
-          const uint64_t key = page[u] >= 0 ? order_of(v) : kLowest;
-          best[k] = r0 == 0 ? key : max(best[k], key);
+        for (int u = 0; u < AT_ONCE; ++u) {
+          double sum[kScoreRows] = {};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const double l = EL::to_f((uint16_t)l_now[u][e]), g = EL::to_f((uint16_t)h_now[u][e]);
+#pragma unroll
+            for (int r = 0; r < kScoreRows; ++r) {
+              sum[r] = __builtin_fma(pos[r][e], g, sum[r]);
+              sum[r] = __builtin_fma(neg[r][e], l, sum[r]);
+            }
+          }
+          // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
+          const bool odd = lane & 1, two = lane & 2;
+          double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
+          u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
+          u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
+          double v = two ? u1 : u0;
+          v += __shfl_xor(two ? u0 : u1, 2, 64);
+#pragma unroll
+          for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
+          if (v != v) v = __builtin_inf();
+          v = fmax(v, __shfl_xor(v, 1, 64));
+          v = fmax(v, __shfl_xor(v, 2, 64));
+          if (c == 0) {
+            const int k = j * OWN * WAVES + wave * OWN + (i0 + u) * BPW + sub;  // block, within the workgroup's
+            const uint64_t key = p_now[u] >= 0 ? order_of(v) : kLowest;
+            best[k] = r0 == 0 ? key : max(best[k], key);
+          }
         }
       }
     }
   }
   __syncthreads();
-  if (tid < kScoreBlocks && first + tid < n) {
-    const int blk = first + tid;
+  for (int k = tid; k < here; k += kScoreThreads) {
+    const int blk = first + k;
     const bool always = blk < a.p.keep_first || blk >= n - a.p.keep_last;
-    a.keys[((int64_t)b * a.p.heads_kv + h) * a.p.max_blocks + blk] = always ? kAlways : best[tid];
+    a.keys[((int64_t)b * a.p.heads_kv + h) * a.p.max_blocks + blk] = always ? kAlways : best[k];
   }
 }
 
 namespace {
-constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64;
+constexpr int kTopThreads = 1024, kTopWaves = kTopThreads / 64;
 constexpr int kDigit = 12, kBins = 1 << kDigit;
 }  // namespace
 
@@ -645,14 +744,18 @@ __global__ __launch_bounds__(kTopThreads) void paged_top_kernel(SelectArgs a) {
     auto count = [&](uint64_t k, bool there) {
       const bool in = there && (top == 64 || (k >> top) == (prefix >> top));
       const uint32_t bin = (uint32_t)(k >> low) & ((1u << width) - 1);
-      // Scores share their leading digit: one atomic for the lanes of the
-      // first lane's bin.
+      // Scores share their leading digits: one atomic for all lanes of a bin,
+      // for the first two bins.
       uint64_t rest = __builtin_amdgcn_ballot_w64(in);
-      if (!rest) return;
-      const uint32_t lead = __shfl(bin, __builtin_ctzll(rest), 64);
-      const uint64_t same = __builtin_amdgcn_ballot_w64(in && bin == lead);
-      if (lane == __builtin_ctzll(rest)) atomicAdd(&bins[lead], (uint32_t)__builtin_popcountll(same));
-      if (in && bin != lead) atomicAdd(&bins[bin], 1u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!rest) return;
+        const int lead = __builtin_ctzll(rest);
+        const uint64_t same = __builtin_amdgcn_ballot_w64(bin == (uint32_t)__builtin_amdgcn_readlane((int)bin, lead)) & rest;
+        if (lane == lead) atomicAdd(&bins[bin], (uint32_t)__builtin_popcountll(same));
+        rest &= ~same;
+      }
+      if ((rest >> lane) & 1u) atomicAdd(&bins[bin], 1u);
     };
     if constexpr (PER) {
 #pragma unroll
@@ -747,7 +850,7 @@ size_t select_workspace_bytes(int batch, int heads_kv, int max_blocks) {
 
 template <typename Tag>
 static hipError_t select_by_dim(const SelectArgs& a, hipStream_t stream) {
-  const dim3 grid((a.p.max_blocks + kScoreBlocks - 1) / kScoreBlocks, a.p.heads_kv, a.p.batch);
+  const dim3 grid((a.p.max_blocks + a.span - 1) / a.span, a.p.heads_kv, a.p.batch);
   const dim3 block(kScoreThreads);
   switch (a.p.head_dim) {
     case 32: hipLaunchKernelGGL((paged_score_kernel<Tag, 32>), grid, block, 0, stream, a); break;
@@ -765,13 +868,18 @@ hipError_t launch_select(const fa_select_params& p, hipStream_t stream) {
   a.p = p;
   a.keys = reinterpret_cast<uint64_t*>(p.workspace);
   a.shift = log2_of(p.block_size);
+  // A workgroup's blocks: 64 while that leaves it company on a compute unit,
+  // then more, so that fewer of them convert their rows again.
+  a.span = 64;
+  const int64_t all = (int64_t)p.batch * p.heads_kv * p.max_blocks;
+  while (a.span < kScoreMost && all / a.span > 8 * (int64_t)device_cu_count()) a.span *= 2;
   if (p.max_blocks > p.n_index) {
     const hipError_t e = p.dtype == FA_DTYPE_F16 ? select_by_dim<f16_t>(a, stream) : select_by_dim<bf16_t>(a, stream);
     if (e != hipSuccess) return e;
   }
   const dim3 grid(p.heads_kv, p.batch);
-  if (p.max_blocks <= 4 * kTopThreads) hipLaunchKernelGGL(paged_top_kernel<4>, grid, dim3(kTopThreads), 0, stream, a);
-  else if (p.max_blocks <= 16 * kTopThreads) hipLaunchKernelGGL(paged_top_kernel<16>, grid, dim3(kTopThreads), 0, stream, a);
+  if (p.max_blocks <= kTopThreads) hipLaunchKernelGGL(paged_top_kernel<1>, grid, dim3(kTopThreads), 0, stream, a);
+  else if (p.max_blocks <= 4 * kTopThreads) hipLaunchKernelGGL(paged_top_kernel<4>, grid, dim3(kTopThreads), 0, stream, a);
   else hipLaunchKernelGGL(paged_top_kernel<0>, grid, dim3(kTopThreads), 0, stream, a);
   return hipGetLastError();
 }
