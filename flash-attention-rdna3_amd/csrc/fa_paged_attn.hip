@@ -30,9 +30,13 @@ PageMode page_mode(const fa_paged_blocks_params& p) {
   return !plain || p.block_size < 16 ? kAnyPages : p.block_size == 16 ? kTwoPages : kOnePage;
 }
 
+// Packed query rows of a KV head above which the kernel for many rows runs.
+constexpr int kManyRows = 32;
+
 struct Plan {
   PageMode pages;
   int r;  // row blocks of 16 that a wave holds: two share the loads and the conversion of a chunk
+  bool many_rows;  // the kernel of fa_paged_rows.hip
   int nrb, rb_rows, shares, head_shift;
 };
 
@@ -40,13 +44,17 @@ Plan plan_of(const fa_paged_blocks_params& p) {
   Plan w;
   w.pages = page_mode(p);
   const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
-  w.r = p.kv_format == FA_KV_SAME || p.head_dim > 128 || w.pages == kAnyPages || rows <= 16 ? 1 : 2;
-  w.nrb = (int)((rows + 16 * w.r - 1) / (16 * w.r));
-  w.rb_rows = (int)std::min<int64_t>(rows, 16 * w.r);
-  w.head_shift = head_shift(p, 8);  // (rows below 256 bytes: 8 waves)
+  const bool eight = p.kv_format != FA_KV_SAME;
+  w.r = !eight || p.head_dim > 128 || w.pages == kAnyPages || rows <= 16 ? 1 : 2;
+  w.many_rows = eight && w.pages != kAnyPages && (p.head_dim == 64 || p.head_dim == 128) && rows > kManyRows;
+  const int rb = w.many_rows ? kRowsBlock : 16 * w.r;
+  w.nrb = (int)((rows + rb - 1) / rb);
+  w.rb_rows = (int)std::min<int64_t>(rows, rb);
+  w.head_shift = w.many_rows ? 0 : head_shift(p, 8);  // (rows below 256 bytes: 8 waves)
+  // One workgroup of 8 waves, or two of 4, for each compute unit.
   const int64_t columns = (int64_t)(p.heads_kv >> w.head_shift) * w.nrb;
-  w.shares = p.shares > 0 ? p.shares
-                          : (int)std::max<int64_t>(1, (device_cu_count() + columns - 1) / columns);
+  const int64_t room = (int64_t)device_cu_count() * (w.many_rows ? 2 : 1);
+  w.shares = p.shares > 0 ? p.shares : (int)std::max<int64_t>(1, (room + columns - 1) / columns);
   return w;
 }
 
@@ -64,7 +72,7 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3((unsigned)(columns * w.shares)), dim3(C::NT), C::LDS_BYTES, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.tickets || w.shares == 1) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
+  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, 5, 2 * C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
@@ -143,6 +151,7 @@ hipError_t launch_paged_blocks(const fa_paged_blocks_params& p, hipStream_t s) {
   a.ws_ml = a.ws_o + partial_rows(p, w) * p.head_dim;
   // (The merge in the same launch addresses partials by 32-bit offsets.)
   a.tickets = partial_rows(p, w) * p.head_dim * 4 < (int64_t(1) << 31) ? p.tickets : nullptr;
+  if (w.many_rows) return launch_paged_rows(a, p.kv_format, p.head_dim, w.nrb, s);
   // (8-bit caches: the kernels' products are fp16 for either query type.)
   switch (p.kv_format) {
     case FA_KV_E4M3: return run_format<f16_t, FA_KV_E4M3>(a, w, p.head_dim, s);

@@ -72,6 +72,12 @@ struct PagedAttnArgs {
   uint32_t* tickets;
 };
 
+// The kernel for many query rows (fa_paged_rows.hip): 8-bit caches, head dim 64
+// or 128, pages of 16 keys or more; a.shares workgroups for each KV head and
+// each of `nrb` blocks of kRowsBlock rows.
+constexpr int kRowsBlock = 128;
+hipError_t launch_paged_rows(const PagedAttnArgs& a, int kv_format, int head_dim, int nrb, hipStream_t stream);
+
 // How a chunk finds its pages.  Strides below 2^31 bytes, one page for its 32
 // keys or one for each half: scalar loads and 32-bit products.  Else each lane
 // finds the page of a key of its own.
@@ -157,6 +163,7 @@ struct Shares {
 struct PagedWork {
   const PagedAttnArgs& a;
   int rb_rows, rb;  // rows of a row block, and the row block
+  int unit;         // log2 of a chunk's keys
   __device__ int length(int b) const {
     const int64_t cap = min((int64_t)a.max_blocks << a.shift, (int64_t)INT_MAX);
     return (int)min((int64_t)max(a.lens[b * a.lens_stride], 0), cap);
@@ -173,7 +180,7 @@ struct PagedWork {
       const int last = r0 / a.seqlen_q == r1 / a.seqlen_q ? r1 % a.seqlen_q : a.seqlen_q - 1;
       n = n - a.seqlen_q + last + 1;
     }
-    return (int)max((n + 31) >> 5, (int64_t)1);
+    return (int)max((n + (1 << unit) - 1) >> unit, (int64_t)1);
   }
   // Every wave computes these alike, 64 sequences at a time.
   __device__ Shares shares(int lane, int least) const {
@@ -245,14 +252,14 @@ __device__ inline int64_t partial_row(const PagedAttnArgs& a, int slot, int hk, 
 
 // Merges the partials of one (sequence, head group, row block): those of the
 // workgroups j0 .. j1, the first of them in its second slot.
-template <int D, int NT, bool AGENT>
+template <int D, bool AGENT>
 __device__ inline void merge_partials(const PagedAttnArgs& a, int b, int hg, int rb, int nrb, int rb_rows, int j0, int j1,
-                                      int tid) {
+                                      int tid, int threads) {
   const int rows = a.heads_q / a.heads_kv * a.seqlen_q, heads = 1 << a.head_shift;
   const int here = min(rb_rows, rows - rb * rb_rows);
   const __amdgpu_buffer_rsrc_t ro = rsrc_of(a.ws_o), rm = rsrc_of(a.ws_ml);
   typedef float f32x2a __attribute__((ext_vector_type(2)));
-  for (int i = tid; i < heads * here * (D / 4); i += NT) {
+  for (int i = tid; i < heads * here * (D / 4); i += threads) {
     const int d = i % (D / 4) * 4, r = i / (D / 4) % here, hk = hg * heads + i / (D / 4 * here);
     float M = kFloor, L = 0.f;
     f32x4a o = {0.f, 0.f, 0.f, 0.f};
@@ -321,7 +328,7 @@ __device__ inline void arrive(const PagedAttnArgs& a, const SharePlace& w, const
     *flag = last;
   }
   __syncthreads();
-  if (*flag) merge_partials<D, NT, true>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, tid);
+  if (*flag) merge_partials<D, true>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, tid, NT);
 }
 
 // A query row of bfloat16 in a lane's s16x8 pieces -> fp16, scaled by a power
@@ -362,7 +369,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
   // The group's heads, each on `streams` waves.
   const int streams = C::NW >> a.head_shift, hw = wave & ((1 << a.head_shift) - 1), stream = wave >> a.head_shift;
   const int hk = (w.hg << a.head_shift) + hw;
-  const PagedWork work{a, w.rb_rows, w.rb};
+  const PagedWork work{a, w.rb_rows, w.rb, 5};
   const Shares cut = work.shares(lane, 2 * streams);
   if (w.share >= cut.count) return;
   const int begin = cut.begin(w.share), end = cut.begin(w.share + 1);
@@ -877,20 +884,23 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
   }
 }
 
-// The merge as a launch of its own: grid (KV heads * row blocks, batch).
-// NW: the waves of the kernel that wrote the partials.
-template <int D, int RB, int NW>
+// The merge as a launch of its own: grid (head groups * row blocks, batch, any).
+// RB, UNIT and LEAST: rows of a row block, log2 of a chunk's keys and fewest
+// chunks of a share (with one KV head; less with more) of the kernel that wrote
+// the partials.
+template <int D, int RB, int UNIT, int LEAST>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, b = blockIdx.y;
   const SharePlace w(a, RB);
-  const PagedWork work{a, w.rb_rows, w.rb};
-  const Shares cut = work.shares(lane, 2 * (NW >> a.head_shift));
+  const PagedWork work{a, w.rb_rows, w.rb, UNIT};
+  const Shares cut = work.shares(lane, LEAST >> a.head_shift);
   int begin = 0;
   for (int b0 = 0; b0 < b; b0 += 64) begin += b0 + lane < b ? work.chunks(b0 + lane) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) begin += __shfl_xor(begin, o, 64);
   const int j0 = cut.owner(begin), j1 = cut.owner(begin + work.chunks(b) - 1);
-  if (j0 != j1) merge_partials<D, 256, false>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, threadIdx.x);
+  if (j0 != j1)
+    merge_partials<D, false>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
 }
 
 }  // namespace fa

@@ -61,7 +61,7 @@ def _bound(c, want, causal):
     ks, vs, index = f("ks"), f("vs"), None if c["index"] is None else c["index"].numpy()
     n = max(n, 0 if index is None else index.shape[2] * k.shape[1])
     near = oracle.attend(q, k, v, c["table"].numpy(), c["lens"].tolist(), ks, vs, index, causal)
-    key = (np.abs(k).max() if ks is None else (np.abs(k).max((1, 3)) * ks).max())
+    key = (np.abs(k).max() if ks is None else (np.abs(k).max((1, 3)) * np.abs(ks)).max())
     logit = (dim + 8) * 2.0 ** -24 * np.abs(q).sum(-1, keepdims=True) * key / np.sqrt(dim)
     out = ROUNDING[c["q"].dtype]
     p = 2.0 ** -11 if c["kind"] in CACHES else out
@@ -98,6 +98,31 @@ def test_block_scales(kind, dtype, heads, kv_heads, rows, dim, block, lens):
 @pytest.mark.parametrize("heads,kv_heads,rows,dim", [(8, 2, 1, 128), (4, 2, 3, 64), (2, 1, 20, 32), (2, 2, 1, 256)])
 def test_small_pages(kind, block, heads, kv_heads, rows, dim):
     _check(_case(block + dim, kind, torch.float16, 3, heads, kv_heads, rows, dim, block, [150, 33, rows]))
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kv_heads,rows,dim,block,lens,n_index", [
+    (8, 2, 33, 128, 16, [300, 33, 64], 0), (4, 1, 64, 128, 32, [500, 64, 65, 700], 0), (2, 2, 129, 64, 64, [129, 200], 0),
+    (5, 1, 50, 64, 128, [1000, 51], 0), (4, 2, 70, 128, 256, [300, 257], 0), (4, 1, 100, 64, 16, [1500, 100], 11),
+    (8, 1, 16, 128, 64, [3000, 16, 17, 900], 5)])
+def test_many_rows(kind, dtype, heads, kv_heads, rows, dim, block, lens, n_index):
+    c = _case(dim + rows, kind, dtype, len(lens), heads, kv_heads, rows, dim, block, lens, n_index)
+    _check(c)
+    _check(c, causal=False, num_splits=3)
+    c["table"][0, 1] = -1
+    c["table"][-1, 0] = 10 ** 9
+    c["q"] = c["q"] * 8
+    _check(c)
+
+
+def test_many_rows_keep_low_logits():
+    # every logit far below zero: the first maximum is not 0
+    c = _case(30, "int8", torch.float16, 2, 4, 1, 40, 64, 16, [400, 60])
+    c["q"], c["k"] = -c["q"].abs() * 30, c["k"].clamp(min=1)
+    _check(c)
+    c["ks"] *= -1  # and far above
+    _check(c)
 
 
 def test_small_pages_wide_heads():
