@@ -16,9 +16,10 @@ namespace fa {
 // [0, first_b) and needs [first_b, last_b), first_b = ceil(min(ctx, cap) / P),
 // last_b = ceil(min(ctx + new, cap) / P); its new blocks are the free list's
 // entries [start_b, start_b + last_b - first_b), start_b the running sum of
-// what the sequences before it need.  The first position of a new block is
-// always a new token (first_b * P >= ctx), so the thread of that token enters
-// the block into the table: no thread reads an entry that another one writes.
+// what the sequences before it need.  Threads of the slot map read the entries
+// below first_b only, and find the others in the free list: no thread reads an
+// entry that another one writes.  What is done is bounded by the tensors' sizes
+// (num_tokens slots, batch * max_blocks entries), whatever the lengths say.
 //
 // One launch, no communication between workgroups: each sums the lengths
 // again (8 bytes a sequence, from L2 after the first) in windows of kSeqs
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(kAllocThreads) void paged_allocate_kernel(fa_alloca
   const int64_t head = p.free_head ? max(*p.free_head, 0) : 0;
   const int64_t stride = (int64_t)gridDim.x * kAllocThreads;
   int64_t tok_base = 0, blk_base = 0;
-  int64_t t = (int64_t)blockIdx.x * kAllocThreads + tid;  // this thread's next token
+  int64_t t = (int64_t)blockIdx.x * kAllocThreads + tid, u = t;  // this thread's next token and block
   for (int b0 = 0; b0 < p.batch; b0 += kSeqs) {
     constexpr int PER = kSeqs / kAllocThreads;
     int64_t tok[PER], blk[PER], tsum = 0, bsum = 0;
@@ -79,12 +80,25 @@ __global__ __launch_bounds__(kAllocThreads) void paged_allocate_kernel(fa_alloca
     __syncthreads();
     if (blockIdx.x == 0) {
       if (b0 == 0 && tid == 0) p.cu_seqlens[0] = 0;
-      for (int i = tid; i < kSeqs && b0 + i < p.batch; i += kAllocThreads) p.cu_seqlens[b0 + i + 1] = (int32_t)tok_end[i];
+      for (int i = tid; i < kSeqs && b0 + i < p.batch; i += kAllocThreads) p.cu_seqlens[b0 + i + 1] = (int32_t)min(tok_end[i], (int64_t)INT32_MAX);
     }
     tok_base += tall;
     blk_base += ball;
-    for (; t < tok_base; t += stride) {
-      int lo = 0, hi = min(kSeqs, p.batch - b0) - 1;  // the first sequence that ends past t
+    const int seqs = min(kSeqs, p.batch - b0);
+    for (; u < blk_base; u += stride) {
+      int lo = 0, hi = seqs - 1;  // the last sequence that starts at or before u: the one that needs it
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (blk_start[mid] <= u) lo = mid;
+        else hi = mid - 1;
+      }
+      const int b = b0 + lo;
+      const int64_t first = (min((int64_t)max(p.context_lens[b * p.context_lens_stride], 0), cap) + P - 1) >> shift;
+      p.block_table[b * p.block_table_stride[0] + (first + u - blk_start[lo]) * p.block_table_stride[1]] =
+          head + u < p.num_free ? p.free_blocks[(head + u) * p.free_blocks_stride] : -1;
+    }
+    for (; t < min(tok_base, (int64_t)p.num_tokens); t += stride) {
+      int lo = 0, hi = seqs - 1;  // the first sequence that ends past t
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (tok_end[mid] > t) hi = mid;
@@ -97,23 +111,21 @@ __global__ __launch_bounds__(kAllocThreads) void paged_allocate_kernel(fa_alloca
       int64_t slot = -1;
       if (pos < cap) {
         const int64_t blk_at = pos >> shift, first = (min(ctx, cap) + P - 1) >> shift;
-        int32_t* const entry = p.block_table + b * p.block_table_stride[0] + blk_at * p.block_table_stride[1];
-        int32_t page;
+        int32_t page = -1;
         if (blk_at < first) {
-          page = *entry;
+          page = p.block_table[b * p.block_table_stride[0] + blk_at * p.block_table_stride[1]];
         } else {
           const int64_t at = head + blk_start[lo] + (blk_at - first);
-          page = at < p.num_free ? p.free_blocks[at * p.free_blocks_stride] : -1;
-          if ((pos & (P - 1)) == 0) *entry = page;
+          if (at < p.num_free) page = p.free_blocks[at * p.free_blocks_stride];
         }
         if (page >= 0) slot = (int64_t)page * P + (pos & (P - 1));
       }
-      if (t < p.num_tokens) p.slots[t] = slot;
+      p.slots[t] = slot;
     }
     __syncthreads();  // the next window writes the arrays
   }
   for (; t < p.num_tokens; t += stride) p.slots[t] = -1;
-  if (blockIdx.x == 0 && tid == 0) p.next_head[0] = (int32_t)(head + blk_base);
+  if (blockIdx.x == 0 && tid == 0) p.next_head[0] = (int32_t)min(head + blk_base, (int64_t)INT32_MAX);
 }
 
 static int log2_of(int n) {

@@ -55,7 +55,7 @@ def paged_kvcache_allocate(block_table, context_lens, new_lens, free_blocks, *, 
         ``max_blocks``); int32 ``(batch + 1,)`` running sums of the new
         lengths, as :func:`flash_attention_varlen` takes them; int32 ``(1,)``
         ``free_head`` for the next call (beyond ``n`` by the blocks that were
-        missing).  ``context_lens`` and ``free_head`` are not modified, and
+        missing).  The sums and ``next_head`` stop at 2^31 - 1.  ``context_lens`` and ``free_head`` are not modified, and
         the same call again gives the same tables.
     """
     validate_block_size(block_size)

@@ -367,7 +367,7 @@ typedef struct fa_paged_blocks_params {
  * entries are -1, and so are the slots of tokens without a page, of tokens
  * past max_blocks * block_size and of rows past the last token.
  * cu_seqlens (batch + 1) are the running sums of the new lengths; next_head is
- * head plus the blocks that were asked for.
+ * head plus the blocks that were asked for; both stop at 2^31 - 1.
  */
 typedef struct fa_allocate_params {
   int32_t abi_version;

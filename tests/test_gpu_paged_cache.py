@@ -63,6 +63,26 @@ def test_allocate_edges():
     _allocate([[-1, 5], [6, 7]], [2, 7], [3, 30], [11], -2, 4, 40)
 
 
+def test_allocate_of_lengths_without_bound():
+    # The work is the tensors', not the lengths': each sequence asks for 2^31 - 1
+    # tokens and gets its table's 8 blocks, while the list lasts; sums stop at 2^31 - 1.
+    top = 2 ** 31 - 1
+    table = torch.full((300, 8), 5, dtype=torch.int32, device=DEVICE)
+    free = torch.arange(2000, dtype=torch.int32, device=DEVICE)
+    slots, cu, nxt = paged_kvcache_allocate(table, torch.zeros(300, dtype=torch.int32, device=DEVICE),
+                                            torch.full((300,), top, dtype=torch.int32, device=DEVICE), free,
+                                            block_size=16, num_tokens=200)
+    torch.testing.assert_close(table.flatten().cpu(), torch.where(torch.arange(2400) < 2000, torch.arange(2400), -1).int())
+    assert slots.tolist() == list(range(128)) + [-1] * 72
+    assert cu.tolist() == [0] + [top] * 300
+    assert nxt.item() == 2400
+    head = int32([top - 5]).to(DEVICE)
+    nxt = paged_kvcache_allocate(table, torch.zeros(300, dtype=torch.int32, device=DEVICE),
+                                 torch.full((300,), 20, dtype=torch.int32, device=DEVICE), free, free_head=head,
+                                 block_size=16, num_tokens=6000)[2]
+    assert nxt.item() == top
+
+
 def test_allocate_strided_and_repeated():
     wide = torch.full((3, 8), 77, dtype=torch.int32, device=DEVICE)
     table = wide[:, ::2]
