@@ -594,6 +594,24 @@ __device__ inline uint64_t order_of(double x) {
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
 
+// x of lane ^ X, for X below 16 within the vector unit: through LDS the steps of
+// a sum wait for one another (32 x 8 x 2048 blocks of D = 128: 75 us against 67,
+// and 64 with the reads sharing the steps as well).
+template <int X> __device__ inline int of_lane_xor(int x) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);  // quad_perm 1 0 3 2
+  else if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);  // quad_perm 2 3 0 1
+  else if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(x, 0x128, 0xF, 0xF, true);  // row_ror 8
+  else if constexpr (X == 4) {
+    const int up = __builtin_amdgcn_mov_dpp(x, 0x104, 0xF, 0xF, true);  // row_shl 4: of lane + 4
+    return __builtin_amdgcn_update_dpp(up, x, 0x114, 0xF, 0xA, true);   // row_shr 4, odd groups of 4
+  } else return __shfl_xor(x, X, 64);
+}
+template <int X> __device__ inline double of_lane_xor(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x);
+  const uint64_t lo = (uint32_t)of_lane_xor<X>((int)b), hi = (uint32_t)of_lane_xor<X>((int)(b >> 32));
+  return __longlong_as_double((long long)(hi << 32 | lo));
+}
+
 __device__ inline int blocks_of(const SelectArgs& a, int b) {
   const int64_t len = max(a.p.context_lens[b * a.p.context_lens_stride], 0);
   return (int)min((int64_t)a.p.max_blocks, (len + a.p.block_size - 1) >> a.shift);
@@ -672,6 +690,11 @@ __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a
           pages_next = pages_of(j + 2);
         }
         ask(pages, turn ? 0 : i0 + AT_ONCE);
+        // A lane's share of the sums, then the sums over the block's lanes, halved
+        // at each step by what a lane keeps: by bit 0 rows {0, 1} or {2, 3}, by bit
+        // 1 one of the two, by bits 2 and 3 one of the reads.
+        double v[AT_ONCE];
+        const bool odd = lane & 1, two = lane & 2, four = lane & 4, eight = lane & 8;
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
           double sum[kScoreRows] = {};
@@ -684,23 +707,35 @@ __global__ __launch_bounds__(kScoreThreads) void paged_score_kernel(SelectArgs a
               sum[r] = __builtin_fma(neg[r][e], l, sum[r]);
             }
           }
-          // Lane bit 0 keeps rows {0, 1} or {2, 3}, bit 1 one of the two.
-          const bool odd = lane & 1, two = lane & 2;
-          double u0 = odd ? sum[2] : sum[0], u1 = odd ? sum[3] : sum[1];
-          u0 += __shfl_xor(odd ? sum[0] : sum[2], 1, 64);
-          u1 += __shfl_xor(odd ? sum[1] : sum[3], 1, 64);
-          double v = two ? u1 : u0;
-          v += __shfl_xor(two ? u0 : u1, 2, 64);
+          double x[2];
 #pragma unroll
-          for (int o = 4; o < LPB; o <<= 1) v += __shfl_xor(v, o, 64);
-          if (v != v) v = __builtin_inf();
-          v = fmax(v, __shfl_xor(v, 1, 64));
-          v = fmax(v, __shfl_xor(v, 2, 64));
-          if (c == 0) {
-            const int k = j * OWN * WAVES + wave * OWN + (i0 + u) * BPW + sub;  // block, within the workgroup's
-            const uint64_t key = p_now[u] >= 0 ? order_of(v) : kLowest;
-            best[k] = r0 == 0 ? key : max(best[k], key);
-          }
+          for (int i = 0; i < 2; ++i) x[i] = (odd ? sum[i + 2] : sum[i]) + of_lane_xor<1>(odd ? sum[i] : sum[i + 2]);
+          v[u] = (two ? x[1] : x[0]) + of_lane_xor<2>(two ? x[0] : x[1]);
+        }
+        int at = 0;  // the read whose sum this lane keeps
+        if constexpr (AT_ONCE > 1) {
+          constexpr int HALF = AT_ONCE / 2;
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) v[i] = (four ? v[i + HALF] : v[i]) + of_lane_xor<4>(four ? v[i] : v[i + HALF]);
+          at = four ? HALF : 0;
+        }
+        if constexpr (AT_ONCE > 2) {
+          v[0] = (eight ? v[1] : v[0]) + of_lane_xor<8>(eight ? v[0] : v[1]);
+          at += eight ? 1 : 0;
+        }
+        if constexpr (LPB > 16) v[0] += of_lane_xor<16>(v[0]);
+        if constexpr (LPB > 32) v[0] += of_lane_xor<32>(v[0]);
+        static_assert(AT_ONCE == (LPB == 4 ? 1 : LPB == 8 ? 2 : 4), "the sums end in one value a lane");
+        double most = v[0] == v[0] ? v[0] : __builtin_inf();
+        most = fmax(most, of_lane_xor<1>(most));
+        most = fmax(most, of_lane_xor<2>(most));
+        int at_page = p_now[0];
+#pragma unroll
+        for (int u = 1; u < AT_ONCE; ++u) at_page = at == u ? p_now[u] : at_page;
+        if ((c & ~(4 * (AT_ONCE - 1))) == 0) {
+          const int k = j * OWN * WAVES + wave * OWN + (i0 + at) * BPW + sub;  // block, within the workgroup's
+          const uint64_t key = at_page >= 0 ? order_of(most) : kLowest;
+          best[k] = r0 == 0 ? key : max(best[k], key);
         }
       }
     }
