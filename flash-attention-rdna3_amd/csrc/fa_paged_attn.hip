@@ -72,7 +72,7 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
   hipLaunchKernelGGL(kern, dim3((unsigned)(columns * w.shares)), dim3(C::NT), C::LDS_BYTES, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.tickets || w.shares == 1) return e;
-  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, 5, 2 * C::NW>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
+  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, 5, C::NW, ShareRule>), dim3((unsigned)columns, (unsigned)a.batch), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }

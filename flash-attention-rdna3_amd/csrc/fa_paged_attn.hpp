@@ -155,14 +155,27 @@ template <int N> __device__ constexpr inline int piece_off(int r, int c) {
 constexpr float kFloor = -3.0e38f;  // the running maximum before any key
 
 // How the chunks of a (head group, row block) are shared out: `total` chunks
-// over `count` workgroups, the first `extra` of them with one more.
+// over `count` workgroups, the first `extra` of them with one more.  `pad` of
+// them are no work: they stand before each sequence's for what its beginning
+// costs.
 struct Shares {
-  int total, count, per, extra;
+  int total, count, per, extra, pad;
   __device__ int begin(int j) const { return j * per + min(j, extra); }
   __device__ int owner(int c) const {
     const int big = extra * (per + 1);
     return c < big ? c / (per + 1) : extra + (c - big) / per;
   }
+};
+
+// A sequence's first chunk waits for its length, table, page and rows in turn: as
+// long as kPad rounds of a workgroup's streams take.  Counted where the sequences
+// have fewer than kPadBelow rounds; longer ones gain nothing by it, and lose the
+// cuts at their ends.  (e4m3, 32/8 heads of 128, 32 sequences up to 2000 keys: 30.5
+// -> 23.1 us, 1 and 2 rounds 25.6 and 24.3; up to 64 x 1200: 40 -> 27.7; 16 lists of
+// 64 blocks of 64, 32 rounds: 33.1, with it 35.2.)
+struct ShareRule {
+  static constexpr int kPad = 3;
+  static constexpr float kPadBelow = 20.f;
 };
 
 struct PagedWork {
@@ -187,24 +200,33 @@ struct PagedWork {
     }
     return (int)max((n + (1 << unit) - 1) >> unit, (int64_t)1);
   }
-  // Every wave computes these alike, 64 sequences at a time.
-  __device__ Shares shares(int lane, int least) const {
+  // Every wave computes these alike, 64 sequences at a time.  A workgroup takes
+  // `streams` chunks at a time, a power of two.
+  template <typename RULE> __device__ Shares shares(int lane, int streams) const {
     Shares s;
     int sum = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) sum += b0 + lane < a.batch ? chunks(b0 + lane) : 0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    s.total = __builtin_amdgcn_readfirstlane(sum);
-    s.count = min(a.shares, max(1, s.total / least));
+    sum = __builtin_amdgcn_readfirstlane(sum);
+    const float steps = (float)sum * __builtin_amdgcn_rcpf((float)(a.batch * streams));  // mean rounds of a sequence
+    s.pad = steps < RULE::kPadBelow ? RULE::kPad * streams - 1 : 0;
+    s.total = sum + s.pad * a.batch;
+    s.count = max(1, min(a.shares, s.total >> __builtin_ctz(2 * streams)));
+    // A sequence's partials are read one after the other, a share's rounds as well:
+    // with fewer shares the one takes less, the other more.  (int8, 3 sequences up to
+    // 6486 keys of 8 heads of 32: 49 us without this limit, with the factor 1, 1.5
+    // and 2 38, 34.3 and 33.5; 4 x 16384 e4m3, 8 heads of 128: 40.2 with 1, else 37.3.)
+    s.count = min(s.count, (int)((float)a.batch * (1.f + 2.f * __builtin_amdgcn_sqrtf(steps))));
     s.per = s.total / s.count;
     s.extra = s.total - s.per * s.count;
     return s;
   }
   // The sequence that holds chunk c, and the chunk it begins at.
-  __device__ void find(int c, int lane, int& b, int& begin) const {
+  __device__ void find(int c, int pad, int lane, int& b, int& begin) const {
     int base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      const int n = b0 + lane < a.batch ? chunks(b0 + lane) : 0;
+      const int n = b0 + lane < a.batch ? chunks(b0 + lane) + pad : 0;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -375,11 +397,11 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
   const int streams = C::NW >> a.head_shift, hw = wave & ((1 << a.head_shift) - 1), stream = wave >> a.head_shift;
   const int hk = (w.hg << a.head_shift) + hw;
   const PagedWork work{a, w.rb_rows, w.rb, 5};
-  const Shares cut = work.shares(lane, 2 * streams);
+  const Shares cut = work.shares<ShareRule>(lane, streams);
   if (w.share >= cut.count) return;
   const int begin = cut.begin(w.share), end = cut.begin(w.share + 1);
   int b, b_begin;
-  work.find(begin, lane, b, b_begin);
+  work.find(begin, cut.pad, lane, b, b_begin);
 
   // This lane's piece of a chunk's first rows.
   typedef const unsigned char* bytes;
@@ -402,7 +424,10 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
 
   for (int at = begin; at < end;) {
     const int len = work.length(b), all = work.chunks(b);
+    b_begin += cut.pad;
+    at = max(at, b_begin);
     const int c0 = at - b_begin, cnt = min(end, b_begin + all) - at;
+    if (cnt <= 0) break;  // (the share ends before the sequence's first chunk)
     const int blocks = (len + mask) >> a.shift;           // logical blocks of the sequence
     const int listed = a.index ? a.n_index : blocks;
     const int32_t* const index = a.index ? a.index + b * a.index_stride[0] + hk * a.index_stride[1] : nullptr;
@@ -904,19 +929,19 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
 }
 
 // The merge as a launch of its own: grid (head groups * row blocks, batch, any).
-// RB, UNIT and LEAST: rows of a row block, log2 of a chunk's keys and fewest
-// chunks of a share (with one KV head; less with more) of the kernel that wrote
-// the partials.
-template <int D, int RB, int UNIT, int LEAST>
+// RB, UNIT and STREAMS: rows of a row block, log2 of a chunk's keys and chunks at
+// a time (with one KV head; less with more) of the kernel that wrote the partials.
+template <int D, int RB, int UNIT, int STREAMS, typename RULE>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   const int lane = threadIdx.x & 63, b = blockIdx.y;
   const SharePlace w(a, RB);
   const PagedWork work{a, w.rb_rows, w.rb, UNIT};
-  const Shares cut = work.shares(lane, LEAST >> a.head_shift);
+  const Shares cut = work.shares<RULE>(lane, STREAMS >> a.head_shift);
   int begin = 0;
   for (int b0 = 0; b0 < b; b0 += 64) begin += b0 + lane < b ? work.chunks(b0 + lane) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) begin += __shfl_xor(begin, o, 64);
+  begin += cut.pad * (b + 1);
   const int j0 = cut.owner(begin), j1 = cut.owner(begin + work.chunks(b) - 1);
   if (j0 != j1)
     merge_partials<D, false>(a, b, w.hg, w.rb, w.nrb, w.rb_rows, j0, j1, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);

@@ -17,13 +17,21 @@ namespace fa {
 template <int D>
 struct RowsCfg {
   static constexpr int NW = 4, NT = 256, RB = kRowsBlock, KEYS = 64, UNIT = 6;
-  static constexpr int LEAST = 8;                  // fewest tiles of a share
+  static constexpr int STREAMS = 4;                // tiles a round counts for: a share has 8 at least
   static constexpr int NSTEP = D / 16, NDB = D / 32;
   static constexpr int PPR = D / 16;               // 16-code pieces of a row
   static constexpr int RPW = 64 / PPR;             // rows a wave loads at a time
   static constexpr int LOADS = KEYS / (NW * RPW);  // loads of a thread
   static constexpr int TILE = KEYS * D;            // elements
   static constexpr int LDS_BYTES = 2 * 2 * TILE * 2 + 16;
+};
+
+// (As in ShareRule, in rounds of four tiles.  int8, 32/8 heads of 128: 16 x 48 rows
+// up to 900 keys 58.6 -> 52.3 us, up to 300 keys 59.5 -> 42; 8 x 200 rows up to 1500
+// keys 110.5 -> 115.9, up to 2500 keys, with no limit, 123.5 -> 136.)
+struct RowsShareRule {
+  static constexpr int kPad = 2;
+  static constexpr float kPadBelow = 4.f;
 };
 
 // PAGES: pages that a tile's 64 keys lie in (1, 2 or 4).
@@ -39,11 +47,11 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnArgs a) {
   const SharePlace w(a, C::RB);
   const int hk = w.hg;
   const PagedWork work{a, w.rb_rows, w.rb, C::UNIT};
-  const Shares cut = work.shares(lane, C::LEAST);
+  const Shares cut = work.shares<RowsShareRule>(lane, C::STREAMS);
   if (w.share >= cut.count) return;
   const int begin = cut.begin(w.share), end = cut.begin(w.share + 1);
   int b, b_begin;
-  work.find(begin, lane, b, b_begin);
+  work.find(begin, cut.pad, lane, b, b_begin);
 
   typedef const unsigned char* bytes;
   typedef const __attribute__((address_space(4))) int32_t const_i32;
@@ -60,7 +68,10 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnArgs a) {
 
   for (int at = begin; at < end;) {
     const int len = work.length(b), all = work.chunks(b);
+    b_begin += cut.pad;
+    at = max(at, b_begin);
     const int c0 = at - b_begin, cnt = min(end, b_begin + all) - at;
+    if (cnt <= 0) break;  // (the share ends before the sequence's first tile)
     const int blocks = (len + mask) >> a.shift;
     const int listed = a.index ? a.n_index : blocks;
     const int32_t* const index = a.index ? a.index + b * a.index_stride[0] + hk * a.index_stride[1] : nullptr;
@@ -363,7 +374,7 @@ hipError_t run_rows(const PagedAttnArgs& a, int nrb, hipStream_t stream) {
   // to merge them than a second launch does (64 rows of 32 heads over 8192 keys,
   // 32 shares: 208 us in all against 48).
   const int rb_rows = std::min(C::RB, a.heads_q / a.heads_kv * a.seqlen_q);
-  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, C::UNIT, C::LEAST>),
+  hipLaunchKernelGGL((paged_merge_kernel<D, C::RB, C::UNIT, C::STREAMS, RowsShareRule>),
                      dim3((unsigned)columns, (unsigned)a.batch, (unsigned)((rb_rows * (D / 4) + 255) / 256)), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
