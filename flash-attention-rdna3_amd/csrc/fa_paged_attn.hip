@@ -30,12 +30,15 @@ PageMode page_mode(const fa_paged_blocks_params& p) {
   return !plain || p.block_size < 16 ? kAnyPages : p.block_size == 16 ? kTwoPages : kOnePage;
 }
 
-// Packed query rows of a KV head above which the kernel for many rows runs.
-constexpr int kManyRows = 32;
+// Packed query rows of a KV head from which the kernel for many rows runs; below,
+// blocks of 16 rows each read the cache again, from L2.  (int8, 32/8 heads of 128,
+// 4 sequences up to 8192 keys: 32 rows 41 us against 42, 48 rows 49 against 43, 64
+// rows 50 against 39; e4m3, 16 up to 2000: 24 rows 27.5 against 45, 48 rows 47.5
+// against 49.5, 64 rows 50 against 35.)
+constexpr int kManyRows = 64;
 
 struct Plan {
   PageMode pages;
-  int r;  // row blocks of 16 that a wave holds: two share the loads and the conversion of a chunk
   bool many_rows;  // the kernel of fa_paged_rows.hip
   int nrb, rb_rows, shares, head_shift;
 };
@@ -45,9 +48,8 @@ Plan plan_of(const fa_paged_blocks_params& p) {
   w.pages = page_mode(p);
   const int64_t rows = (int64_t)(p.heads_q / p.heads_kv) * p.seqlen_q;
   const bool eight = p.kv_format != FA_KV_SAME;
-  w.r = !eight || p.head_dim > 128 || w.pages == kAnyPages || rows <= 16 ? 1 : 2;
-  w.many_rows = eight && w.pages != kAnyPages && (p.head_dim == 64 || p.head_dim == 128) && rows > kManyRows;
-  const int rb = w.many_rows ? kRowsBlock : 16 * w.r;
+  w.many_rows = eight && w.pages != kAnyPages && (p.head_dim == 64 || p.head_dim == 128) && rows >= kManyRows;
+  const int rb = w.many_rows ? kRowsBlock : 16;
   w.nrb = (int)((rows + rb - 1) / rb);
   w.rb_rows = (int)std::min<int64_t>(rows, rb);
   w.head_shift = w.many_rows ? 0 : head_shift(p, 8);  // (rows below 256 bytes: 8 waves)
@@ -62,10 +64,10 @@ int64_t partial_rows(const fa_paged_blocks_params& p, const Plan& w) {
   return 2 * (int64_t)w.shares * p.heads_kv * w.nrb * w.rb_rows;
 }
 
-template <typename Tag, int KV, int D, int R, int PAGES>
+template <typename Tag, int KV, int D, int PAGES>
 hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
-  using C = AttnCfg<Tag, KV, D, R, PAGES>;
-  auto kern = paged_attn_kernel<Tag, KV, D, R, PAGES>;
+  using C = AttnCfg<Tag, KV, D, PAGES>;
+  auto kern = paged_attn_kernel<Tag, KV, D, PAGES>;
   hipError_t e = allow_lds((const void*)kern, C::LDS_BYTES);
   if (e != hipSuccess) return e;
   const int columns = (a.heads_kv >> a.head_shift) * w.nrb;
@@ -79,13 +81,12 @@ hipError_t run(PagedAttnArgs a, const Plan& w, hipStream_t stream) {
 
 template <typename Tag, int KV, int D>
 hipError_t run_dim(const PagedAttnArgs& a, const Plan& w, hipStream_t s) {
-  if (w.pages == kAnyPages) return run<Tag, KV, D, 1, kAnyPages>(a, w, s);
-  if constexpr (KV != FA_KV_SAME && D <= 128) {
-    if (w.r == 2 && w.pages == kOnePage) return run<Tag, KV, D, 2, kOnePage>(a, w, s);
-    if (w.r == 2) return run<Tag, KV, D, 2, kTwoPages>(a, w, s);
+  switch (w.pages) {
+    case kOnePage: return run<Tag, KV, D, kOnePage>(a, w, s);
+    case kTwoPages: return run<Tag, KV, D, kTwoPages>(a, w, s);
+    case kAnyPages: return run<Tag, KV, D, kAnyPages>(a, w, s);
   }
-  if (w.pages == kOnePage) return run<Tag, KV, D, 1, kOnePage>(a, w, s);
-  return run<Tag, KV, D, 1, kTwoPages>(a, w, s);
+  return hipErrorInvalidValue;
 }
 
 template <typename Tag, int KV>

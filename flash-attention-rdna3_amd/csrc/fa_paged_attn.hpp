@@ -88,7 +88,7 @@ hipError_t launch_paged_rows(const PagedAttnArgs& a, int kv_format, int head_dim
 // finds the page of a key of its own.
 enum PageMode { kOnePage, kTwoPages, kAnyPages };
 
-template <typename Tag, int KV, int D, int R, int PAGES>
+template <typename Tag, int KV, int D, int PAGES>
 struct AttnCfg {
   static constexpr bool KV8 = KV != FA_KV_SAME;
   static constexpr int ES = KV8 ? 1 : 2;                      // bytes of an element
@@ -98,7 +98,7 @@ struct AttnCfg {
   // Waves: two per SIMD where their registers and tiles have room.
   static constexpr int NW = TILE >= 32768 ? 2 : TILE >= 16384 ? 4 : 8;
   static constexpr int NT = 64 * NW;
-  static constexpr int RB = 16 * R;                           // rows of a row block
+  static constexpr int RB = 16;                               // rows of a row block
   static constexpr int NSTEP = D / 32;                        // 32-dim steps of Q K^T
   static constexpr int NDB = D / 16;                          // 16-dim blocks of O
   static constexpr bool PAIR = KV8 && NSTEP > 1;              // 16 bytes of K serve two steps
@@ -381,9 +381,9 @@ __device__ inline float bf16_row_top(const s16x8 (&q)[N]) {
   return top;
 }
 
-template <typename Tag, int KV, int D, int R, int PAGES>
-__global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_attn_kernel(PagedAttnArgs a) {
-  using C = AttnCfg<Tag, KV, D, R, PAGES>;
+template <typename Tag, int KV, int D, int PAGES>
+__global__ __launch_bounds__((AttnCfg<Tag, KV, D, PAGES>::NT)) void paged_attn_kernel(PagedAttnArgs a) {
+  using C = AttnCfg<Tag, KV, D, PAGES>;
   using CT = typename std::conditional<C::KV8, f16_t, Tag>::type;  // type of the products
   constexpr bool ANY = PAGES == kAnyPages;
   constexpr int NH = PAGES == kTwoPages ? 2 : 1;  // pages a chunk is described by
@@ -533,23 +533,18 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     }
 
     // --- Q -----------------------------------------------------------------
-    s16x8 q[R][C::NSTEP];
-    float qscale[R];
-    int klim[R];
+    s16x8 q[C::NSTEP];
+    const int row = w.rb * C::RB + l16;
+    const bool valid = row < rows;
+    const int g = valid ? row / a.seqlen_q : 0, m = valid ? row - g * a.seqlen_q : 0;
+    const int klim = a.causal ? len - a.seqlen_q + m : INT_MAX;
+    const uint16_t* const src = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_stride[0] +
+                                (hk * group + g) * a.q_stride[1] + m * a.q_stride[2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = w.rb * C::RB + 16 * r + l16;
-      const bool valid = row < rows;
-      const int g = valid ? row / a.seqlen_q : 0, m = valid ? row - g * a.seqlen_q : 0;
-      klim[r] = a.causal ? len - a.seqlen_q + m : INT_MAX;
-      const uint16_t* const src = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_stride[0] +
-                                  (hk * group + g) * a.q_stride[1] + m * a.q_stride[2];
-#pragma unroll
-      for (int s = 0; s < C::NSTEP; ++s) {
-        // With paired K loads, lane group g4 covers 16 dims of a pair of steps.
-        const int d = C::PAIR ? 64 * (s / 2) + 16 * g4 + 8 * (s % 2) : 32 * s + 8 * g4;
-        q[r][s] = valid ? *reinterpret_cast<const s16x8*>(src + d) : zero_op<f16_t>();
-      }
+    for (int s = 0; s < C::NSTEP; ++s) {
+      // With paired K loads, lane group g4 covers 16 dims of a pair of steps.
+      const int d = C::PAIR ? 64 * (s / 2) + 16 * g4 + 8 * (s % 2) : 32 * s + 8 * g4;
+      q[s] = valid ? *reinterpret_cast<const s16x8*>(src + d) : zero_op<f16_t>();
     }
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
@@ -558,37 +553,28 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     }
     Meta ahead = describe(chunk(0), first);
     load(ahead);
-    float zero[R];  // first value of Q K^T's sums
+    float qscale = a.scale_log2;
+    if (C::KV8 && a.bf16) {
+      float top = bf16_row_top(q);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      qscale *= bf16_row_to_f16(q, top);
+    }
+    float zero = 0.f;  // first value of Q K^T's sums
+    if constexpr (KV == FA_KV_INT8) {
+      const short c = (short)Elem<f16_t>::from_f(-kInt8Offset);
+      const s16x8 off = {c, c, c, c, c, c, c, c};
+      f32x4a x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      qscale[r] = a.scale_log2;
-      if (C::KV8 && a.bf16) {
-        float top = bf16_row_top(q[r]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        qscale[r] *= bf16_row_to_f16(q[r], top);
-      }
-      zero[r] = 0.f;
-      if constexpr (KV == FA_KV_INT8) {
-        const short c = (short)Elem<f16_t>::from_f(-kInt8Offset);
-        const s16x8 off = {c, c, c, c, c, c, c, c};
-        f32x4a x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < C::NSTEP; ++s) x = mma16x16<f16_t>(off, q[r][s], x);
-        zero[r] = x[0];
-      }
+      for (int s = 0; s < C::NSTEP; ++s) x = mma16x16<f16_t>(off, q[s], x);
+      zero = x[0];
     }
 
     // --- the stream ----------------------------------------------------------
-    float m_i[R], l_i[R];
-    f32x4a acc[R][C::NDB];
+    float m_i = kFloor, l_i = 0.f;
+    f32x4a acc[C::NDB];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      m_i[r] = kFloor;
-      l_i[r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < C::NDB; ++i) acc[r][i] = f32x4a{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int i = 0; i < C::NDB; ++i) acc[i] = f32x4a{0.f, 0.f, 0.f, 0.f};
     uint32_t vref = 0x00800000u;  // bits of a power of two
     // Elements that are not finite: (x & ABS) + UP has the top bit set.
     constexpr uint32_t ABS = C::KV8 ? 0x7F7F7F7Fu : 0x7FFF7FFFu;
@@ -641,22 +627,18 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
           later[h] = logical_of(first_key(chunk(k + 3), h));
         }
       }
-      f32x4a s[R][2];
+      f32x4a s[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 16 * h + l16;
-#pragma unroll
-        for (int r = 0; r < R; ++r) s[r][h] = f32x4a{zero[r], zero[r], zero[r], zero[r]};
+        s[h] = f32x4a{zero, zero, zero, zero};
         if constexpr (C::PAIR) {
 #pragma unroll
           for (int t = 0; t < C::NSTEP; t += 2) {
             const u32x4 y = *reinterpret_cast<const u32x4*>(ktile + piece_off<C::PPR>(row, 2 * t + g4));
             const s16x8 lo = codes_to_f16<KV, true>(u32x2{y[0], y[1]}), hi = codes_to_f16<KV, true>(u32x2{y[2], y[3]});
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-              s[r][h] = mma16x16<CT>(lo, q[r][t], s[r][h]);
-              s[r][h] = mma16x16<CT>(hi, q[r][t + 1], s[r][h]);
-            }
+            s[h] = mma16x16<CT>(lo, q[t], s[h]);
+            s[h] = mma16x16<CT>(hi, q[t + 1], s[h]);
           }
         } else {
 #pragma unroll
@@ -666,8 +648,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
               x = codes_to_f16<KV, true>(*reinterpret_cast<const u32x2*>(ktile + piece_off<C::PPR>(row, g4 / 2) + g4 % 2 * 8));
             else
               x = *reinterpret_cast<const s16x8*>(ktile + piece_off<C::PPR>(row, 4 * t + g4));
-#pragma unroll
-            for (int r = 0; r < R; ++r) s[r][h] = mma16x16<CT>(x, q[r][t], s[r][h]);
+            s[h] = mma16x16<CT>(x, q[t], s[h]);
           }
         }
       }
@@ -700,9 +681,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
           const float f = __uint_as_float((uint32_t)max((int)(0x3F800000u + vref - grown), 0));
           vref = grown;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int i = 0; i < C::NDB; ++i) acc[r][i] *= f;
+          for (int i = 0; i < C::NDB; ++i) acc[i] *= f;
         }
         const float inv = __uint_as_float(0x7F000000u - vref);
 #pragma unroll
@@ -722,79 +701,76 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
           }
       }
       const bool masked = ANY || !whole || mixed;
-      s16x8 p[R];
+      s16x8 p;
+      float f[2][NI];  // factor of the logits
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float f[2][NI];  // factor of the logits
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < NI; ++i) f[h][i] = qscale[r] * ks[h][i];
-        uint32_t seen = 0xFFu;  // this lane's keys that its row sees
-        if (masked) {
-          seen = 0;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int pos = ANY ? of_key(m.key0, h, i) : m.key0[NH == 2 ? h : 0] + (NH == 2 ? 0 : 16 * h) + 4 * g4 + i;
-              const bool yes = ((m.there >> (16 * h + 4 * g4 + i)) & 1u) && pos <= klim[r];
-              seen |= yes ? 1u << (4 * h + i) : 0u;
-            }
-        }
-        f32x4a x[2];
-        float top = kNegInf;
+        for (int i = 0; i < NI; ++i) f[h][i] = qscale * ks[h][i];
+      uint32_t seen = 0xFFu;  // this lane's keys that its row sees
+      if (masked) {
+        seen = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[r][h][i], f[h][ANY ? i : 0], -m_i[r]);
-        auto hide = [&]() {
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = (seen >> i) & 1u ? x[i / 4][i % 4] : kNegInf;
+          for (int i = 0; i < 4; ++i) {
+            const int pos = ANY ? of_key(m.key0, h, i) : m.key0[NH == 2 ? h : 0] + (NH == 2 ? 0 : 16 * h) + 4 * g4 + i;
+            const bool yes = ((m.there >> (16 * h + 4 * g4 + i)) & 1u) && pos <= klim;
+            seen |= yes ? 1u << (4 * h + i) : 0u;
           }
-        };
+      }
+      f32x4a x[2];
+      float top = kNegInf;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[h][i], f[h][ANY ? i : 0], -m_i);
+      auto hide = [&]() {
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i / 4][i % 4] = (seen >> i) & 1u ? x[i / 4][i % 4] : kNegInf;
+        }
+      };
+      hide();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i / 4][i % 4]);
+      if (__builtin_amdgcn_ballot_w64(top > 8.f)) {
+        float high = m_i;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            high = fmaxf(high, (seen >> (4 * h + i)) & 1u ? s[h][i] * f[h][ANY ? i : 0] : kNegInf);
+        high = fmaxf(high, __shfl_xor(high, 16, 64));
+        high = fmaxf(high, __shfl_xor(high, 32, 64));
+        const float down = __builtin_amdgcn_exp2f(m_i - high);
+        m_i = high;
+        l_i *= down;
+#pragma unroll
+        for (int i = 0; i < C::NDB; ++i) acc[i] *= down;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[h][i], f[h][ANY ? i : 0], -high);
         hide();
+      }
+      float e[8], y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i / 4][i % 4]);
-        if (__builtin_amdgcn_ballot_w64(top > 8.f)) {
-          float high = m_i[r];
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(x[i / 4][i % 4]);
+        y[i] = C::KV8 ? e[i] * wv[i / 4][ANY ? i % 4 : 0] : e[i];
+      }
+      if (C::KV8 && __builtin_expect(scale_top >= 0x7F800000u, 0)) {  // (0 * a scale that is not finite)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int i = 0; i < 8; ++i) y[i] = x[i / 4][i % 4] == kNegInf ? 0.f : y[i];
+      }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              high = fmaxf(high, (seen >> (4 * h + i)) & 1u ? s[r][h][i] * f[h][ANY ? i : 0] : kNegInf);
-          high = fmaxf(high, __shfl_xor(high, 16, 64));
-          high = fmaxf(high, __shfl_xor(high, 32, 64));
-          const float down = __builtin_amdgcn_exp2f(m_i[r] - high);
-          m_i[r] = high;
-          l_i[r] *= down;
+      for (int i = 0; i < 8; ++i) p[i] = (short)Elem<CT>::from_f(y[i]);
 #pragma unroll
-          for (int i = 0; i < C::NDB; ++i) acc[r][i] *= down;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[h][i] = __builtin_fmaf(s[r][h][i], f[h][ANY ? i : 0], -high);
-          hide();
-        }
-        float e[8], y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(x[i / 4][i % 4]);
-          y[i] = C::KV8 ? e[i] * wv[i / 4][ANY ? i % 4 : 0] : e[i];
-        }
-        if (C::KV8 && __builtin_expect(scale_top >= 0x7F800000u, 0)) {  // (0 * a scale that is not finite)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i / 4][i % 4] == kNegInf ? 0.f : y[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[r][i] = (short)Elem<CT>::from_f(y[i]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float z = Elem<CT>::to_f((uint16_t)p[r][i]);
-          if constexpr (!C::KV8) l_i[r] += z;
-          else l_i[r] += kept[i / 4][ANY ? i % 4 : 0] ? z * back[i / 4][ANY ? i % 4 : 0] : e[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float z = Elem<CT>::to_f((uint16_t)p[i]);
+        if constexpr (!C::KV8) l_i += z;
+        else l_i += kept[i / 4][ANY ? i % 4 : 0] ? z * back[i / 4][ANY ? i % 4 : 0] : e[i];
       }
       // V^T: group g4's slots are the keys 4 g4 + 0 .. 3 and 16 + 4 g4 + 0 .. 3, as
       // in the scores.
@@ -816,8 +792,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
           const s4a hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(t + 16 * D));
           v = s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][i] = mma16x16<CT>(v, p[r], acc[r][i]);
+        acc[i] = mma16x16<CT>(v, p, acc[i]);
       }
     }
     if (KV != FA_KV_INT8 && __builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {
@@ -857,9 +832,7 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
               if constexpr (C::KV8) f = (*at_v & 0x7F) == 0x7F ? __builtin_nanf("") : 0.f;
               else f = Elem<CT>::to_f(*reinterpret_cast<const uint16_t*>(at_v));
               if (f - f == 0.f) continue;
-#pragma unroll
-              for (int r = 0; r < R; ++r)
-                if (pos <= klim[r]) acc[r][i][e] += f * vs;
+              if (pos <= klim) acc[i][e] += f * vs;
             }
         }
       }
@@ -871,19 +844,16 @@ __global__ __launch_bounds__((AttnCfg<Tag, KV, D, R, PAGES>::NT)) void paged_att
     float* const sm = so + C::NW * C::RB * C::OLD;
     float* const sl = sm + C::NW * C::RB;
     __syncthreads();
+    l_i += __shfl_xor(l_i, 16, 64);
+    l_i += __shfl_xor(l_i, 32, 64);
+    const int at_row = wave * C::RB + l16;  // (waves of a head: hw, hw + heads, ...)
+    if (l16 < w.rb_rows) {
+      float* const st = so + at_row * C::OLD + 4 * g4;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      l_i[r] += __shfl_xor(l_i[r], 16, 64);
-      l_i[r] += __shfl_xor(l_i[r], 32, 64);
-      const int row = wave * C::RB + 16 * r + l16;  // (waves of a head: hw, hw + heads, ...)
-      if (16 * r + l16 < w.rb_rows) {
-        float* const st = so + row * C::OLD + 4 * g4;
-#pragma unroll
-        for (int i = 0; i < C::NDB; ++i) *reinterpret_cast<f32x4a*>(st + 16 * i) = acc[r][i] * vscale;
-        if (g4 == 0) {
-          sm[row] = m_i[r];
-          sl[row] = l_i[r];
-        }
+      for (int i = 0; i < C::NDB; ++i) *reinterpret_cast<f32x4a*>(st + 16 * i) = acc[i] * vscale;
+      if (g4 == 0) {
+        sm[at_row] = m_i;
+        sl[at_row] = l_i;
       }
     }
     __syncthreads();
