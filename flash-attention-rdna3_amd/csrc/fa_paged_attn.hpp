@@ -7,7 +7,7 @@
 // One pass over the keys with a running maximum and sum, fp32 throughout.
 //
 //  * Work.  The keys of all sequences are one line of 32-key chunks, cut into
-//    equal shares, one for each workgroup of a (KV head, row block): no
+//    equal shares, one for each workgroup of a (head group, row block): no
 //    workgroup has more than another, whatever the lengths.  A share holds the
 //    end of one sequence, whole ones, and the start of another; sequences that
 //    several shares hold are merged from unnormalised partials by the last
@@ -33,6 +33,9 @@
 //    for there the rounded one may have lost its bits).  It costs nothing here,
 //    36.1 us either way over 134 MB of e4m3; in the kernel of many query rows,
 //    which is bound by its instructions, 225 us against 204: there l sums p.
+//  * What bounds it: the stream.  int8, 4 contexts up to 131072 of 8 heads of 128,
+//    854 MB: 152 us, 5.6 TB/s (a read alone: 7.0); e4m3, 4 x 16384, 134 MB: 35 us,
+//    of which ramp, first chain of loads and merge are some 10.
 //  * The maximum moves only when a logit passes it by more than 8 (in powers
 //    of two): p <= 2^8 is exact enough in fp16, and most chunks then skip the
 //    rescaling.
