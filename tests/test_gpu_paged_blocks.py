@@ -177,6 +177,16 @@ def test_both_merges(fused, rows, monkeypatch):
     _check(_case(6, "int8", torch.float16, 3, 8, 2, rows, 128, 32, [2000, 40, 1111]))
 
 
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,rows,dim,lens", [
+    (8, 8, 1, 32, [1500, 700, 901]),                                # many rounds of a wave: no pads
+    (4, 1, 1, 128, [1] * 40 + [9000] + [0, 33] * 30),               # one long sequence among short ones
+    (8, 1, 20, 64, [20] * 70 + [2500, 64, 65]), (8, 1, 20, 64, [2500, 3100])])  # blocks of many rows
+def test_shares_of_uneven_sequences(fused, heads, kv_heads, rows, dim, lens, monkeypatch):
+    monkeypatch.setattr(_native, "FUSED_SPLIT_MERGE", fused)
+    _check(_case(40 + dim, "int8", torch.float16, len(lens), heads, kv_heads, rows, dim, 32, lens))
+
+
 def test_many_sequences():
     g = torch.Generator().manual_seed(7)
     lens = torch.randint(0, 90, (150,), generator=g).tolist()
